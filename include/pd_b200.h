@@ -220,6 +220,13 @@ int pd_paged_decode_bounded(int dtype, const pd_params* p, int num_pages, void* 
 int pd_paged_decode_scaled(int dtype, const pd_params* p, int num_pages, const float* d_k_scales,
                            const float* d_v_scales, void* stream);
 
+/* The same decode over an e4m3 cache with one scale per (block of tokens, kv head) for K and for V, as
+ * pd_append_qkv and a cache with pd_cache_set_block_scales leave it.  No counterpart in the reference.
+ * d_block_scales: device floats [num_pages][num_kv_heads][page_size / block][2] (K, V), 8-byte aligned, block =
+ * pd_scale_block_tokens(page_size); positive and finite (0: nothing was ever written there).  p->k_scale and
+ * p->v_scale are ignored.  num_pages must be positive: scales of pages outside [0, num_pages) are not read. */
+int pd_paged_decode_block_scaled(int dtype, const pd_params* p, int num_pages, const float* d_block_scales, void* stream);
+
 /* What a decode of these params would launch (no counterpart in the reference, which has one kernel shape):
  * out[0] schedule (0 the caller's plan as bound, 1 the same step cut by rows for the head-fused kernel,
  * 2 the caller's plan cut in unequal shares by the adaptive cut), out[1] grid, out[2] tokens per tile,
@@ -257,7 +264,8 @@ int pd_paged_decode_static(int dtype, const pd_params* p, int num_segments, int 
 
 /* Device status word of the last decode launched by this thread's library state:
  * 0 = every bounded wait completed.  Reads it back (synchronises `stream`).
- * Nonzero encodes (code << 24 | cta) of the first wait that gave up. */
+ * Nonzero encodes (code << 24 | cta) of the first wait that gave up; code 7 (code << 24 | row) comes from an
+ * append whose row had no place in the block table or the pool. */
 int pd_kernel_status(void* stream, unsigned* status);
 
 /* Multi-GPU (no counterpart in the reference, which is single-GPU): the decode layer sharded over
@@ -324,6 +332,89 @@ int pd_append_tokens_scaled(int dtype, const void* d_k, const void* d_v, void* k
                             int head_dim, int page_size, float k_scale, float v_scale,
                             const float* d_k_scales, const float* d_v_scales, void* stream);
 
+/* ---- Rows of q, k and v on their way to the attention (no counterpart in the reference, whose callers norm and
+ * rotate elsewhere and whose append copies) ----
+ *
+ * A rotation (rotary position embedding) of the first rotary_dim dims of every q and k head.  Frequency i < rotary_dim / 2
+ * turns pair i by position * inv_freq[i] radians; pairs are (i, i + rotary_dim/2), or (2i, 2i + 1) with `interleaved`.
+ * axes[i] (0..3; NULL: all 0) is the row of pd_qkv::positions that drives frequency i, for positions with several axes
+ * (time, height, width).  `scale` multiplies sine and cosine (1 for most models).  Angles are exact integer fractions
+ * of a turn, so any int32 position is as accurate as a small one.  rotary_dim: a multiple of 16, 16..128; |inv_freq| <=
+ * 1e6.  A host object: it may be destroyed as soon as the calls it was passed to have returned, captured ones too. */
+typedef enum pd_act_dtype { PD_ACT_FP16 = 0, PD_ACT_BF16 = 1 } pd_act_dtype;
+typedef struct pd_rope pd_rope;
+int  pd_rope_create(int rotary_dim, const double* inv_freq, const int* axes, int interleaved, float scale, pd_rope** out);
+void pd_rope_destroy(pd_rope* rope);
+
+/* The rows of one call.  Token t's heads are num_*_heads * head_dim consecutive elements at q + t * q_stride and so on
+ * (strides in elements, multiples of 8; 0: dense), so q, k and v may be slices of one packed projection.  Pointers
+ * are 16-byte aligned. */
+typedef struct pd_qkv {
+    const void* q;             /* may be NULL with num_q_heads = 0 */
+    const void* k;
+    const void* v;             /* pd_qk_norm_rope ignores it */
+    long long   q_stride;
+    long long   k_stride;
+    long long   v_stride;
+    const void* q_norm;        /* [head_dim] weight of the RMS norm of every q head, in act_dtype; NULL: no norm */
+    const void* k_norm;
+    const int*  positions;     /* device [num_axes][positions_stride]; NULL in an append: the token's place in the cache */
+    long long   positions_stride;
+    int         num_axes;
+    int         act_dtype;     /* pd_act_dtype of q, k, v and the weights */
+    int         num_tokens;
+    int         num_q_heads;
+    int         num_kv_heads;
+    int         head_dim;      /* 128 */
+    float       eps;           /* of the norm: x * w / sqrt(mean(x^2) + eps) */
+} pd_qkv;
+
+/* Norm (where there is a weight) and rotation (rope may be NULL) of the q and k rows in one pass; arithmetic in
+ * fp32, one rounding to act_dtype.  Output strides as in pd_qkv.  In place (q_out == q, k_out == k, same strides) is
+ * allowed; other overlaps are not. */
+int pd_qk_norm_rope(const pd_qkv* x, const pd_rope* rope, void* q_out, long long q_out_stride, void* k_out,
+                    long long k_out_stride, void* stream);
+
+/* Tokens that share a scale in a block-scaled cache: the largest power of two that divides the page size, at most 16. */
+int pd_scale_block_tokens(int page_size);
+
+/* Where pd_append_qkv puts k and v.  Sequence b owns rows [token_begin[b], token_begin[b + 1]) of the call (ascending;
+ * sequences may be empty) and they become its tokens start_pos[b], start_pos[b] + 1, ...  All arrays are read on the
+ * device: nothing is copied from the host, and the call may be captured and replayed while they change.
+ *   - Rows of no sequence (behind the last one: a padded batch) and sequences with a negative slot are skipped: neither
+ *     their pages nor their rows of q_out are touched.
+ *   - A place outside the block table, or a page outside [0, num_pages), is not written; pd_kernel_status then reports
+ *     code 7 with the row.
+ *   - No two sequences of a call may write the same page.
+ *   - fp8 cache: per-tensor scales, d_k_scales / d_v_scales per kv head, or d_block_scales.  The stored byte is
+ *     e4m3(value / scale), rounded once from fp32.
+ *   - d_block_scales [num_pages][num_kv_heads][page_size / block][2] (K, V): every block that receives tokens gets the
+ *     smallest power of two (2^-32 .. 2^8) that brings its largest new magnitude to at most 448; a block that was begun
+ *     by an earlier call keeps its scale if that is larger, otherwise the rest of the block is re-encoded (an
+ *     exponent shift: exact while the values stay normal numbers of e4m3). */
+typedef struct pd_append_target {
+    void*       k_cache;            /* [num_pages][num_kv_heads][page_size][head_dim], fp16 or e4m3 */
+    void*       v_cache;
+    const int*  block_table;        /* [num_slots][block_table_stride] */
+    const int*  start_pos;          /* [batch] tokens of each sequence before this call */
+    const int*  token_begin;        /* [batch + 1]; NULL: one token each, row b is sequence b */
+    const int*  slot_ids;           /* [batch] row of block_table per sequence; NULL = identity */
+    const float* d_k_scales;        /* [num_kv_heads] or NULL */
+    const float* d_v_scales;
+    float*      d_block_scales;     /* or NULL */
+    float       k_scale;
+    float       v_scale;
+    int         block_table_stride;
+    int         num_slots;
+    int         batch;
+    int         num_pages;
+    int         page_size;
+} pd_append_target;
+
+/* Norm, rotation and append in one pass: q leaves as dense fp16 rows [num_tokens][num_q_heads][head_dim] (what the
+ * decode reads), k and v go to their pages.  Does not wait. */
+int pd_append_qkv(int dtype, const pd_qkv* x, const pd_rope* rope, const pd_append_target* t, void* q_out, void* stream);
+
 /* decode::PagedKVCache (src/decode/paged_kv_cache.hpp:31-73). */
 size_t pd_cache_bytes_per_page(const pd_cache_config* cfg);
 int    pd_cache_pages_for_budget(const pd_cache_config* cfg, size_t budget_bytes);
@@ -340,11 +431,23 @@ int    pd_cache_append(pd_cache* c, int slot, const void* d_k, const void* d_v, 
  * wait, and the sources must stay valid until the stream has consumed them. */
 int    pd_cache_append_batch(pd_cache* c, int count, const int* slots, const void* const* d_k,
                              const void* const* d_v, const int* n, void* stream);
+/* pd_append_qkv for slots of the cache, with the allocation rules and the stream order of pd_cache_append_batch: the
+ * rows of `x` are the n[0] tokens of slots[0], then the n[1] of slots[1], ... (together x->num_tokens).  q_out receives
+ * the fp16 query rows.  No counterpart in the reference. */
+int    pd_cache_append_qkv(pd_cache* c, int count, const int* slots, const int* n, const pd_qkv* x, const pd_rope* rope,
+                           void* q_out, void* stream);
 int    pd_cache_release(pd_cache* c, int slot);
 /* Per-kv-head scales for an fp8 cache (host arrays of num_kv_heads positive floats; both NULL: back to
  * the per-tensor scales of the config).  Every later append quantises and every later run dequantises
  * with them.  Only while the cache holds no tokens.  No counterpart in the reference. */
 int    pd_cache_set_head_scales(pd_cache* c, const float* k_scales, const float* v_scales);
+/* One scale per (block of tokens, kv head) for K and for V instead of the config's per-tensor scales (fp8 cache; on = 0:
+ * back to those).  Every later append quantises with them, as pd_append_qkv does, and every later run reads them.
+ * Only while the cache holds no tokens and without head scales.  Adds 8 bytes per block and kv head, which
+ * pd_cache_bytes_per_page and pd_cache_total_bytes do not count.  No counterpart in the reference. */
+int    pd_cache_set_block_scales(pd_cache* c, int on);
+/* The device array (layout of pd_append_target::d_block_scales), or NULL without block scales. */
+float* pd_cache_block_scales(const pd_cache* c);
 void   pd_cache_shuffle_free_pages(pd_cache* c, unsigned seed);
 int    pd_cache_plan(pd_cache* c, const int* slots, int num_slots, int num_q_heads, int num_ctas, void* stream);
 /* plan() through the device-side planner (pd_device_plan_build) from the cache's own device lengths, which

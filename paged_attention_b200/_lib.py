@@ -49,6 +49,26 @@ class pd_cache_config(C.Structure):
     ]
 
 
+class pd_qkv(C.Structure):
+    """The q, k and v rows of one call (no counterpart in the reference)."""
+    _fields_ = [
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("q_stride", C.c_longlong), ("k_stride", C.c_longlong),
+        ("v_stride", C.c_longlong), ("q_norm", C.c_void_p), ("k_norm", C.c_void_p), ("positions", C.c_void_p),
+        ("positions_stride", C.c_longlong), ("num_axes", C.c_int), ("act_dtype", C.c_int), ("num_tokens", C.c_int),
+        ("num_q_heads", C.c_int), ("num_kv_heads", C.c_int), ("head_dim", C.c_int), ("eps", C.c_float),
+    ]
+
+
+class pd_append_target(C.Structure):
+    """Where an append puts k and v (no counterpart in the reference)."""
+    _fields_ = [
+        ("k_cache", C.c_void_p), ("v_cache", C.c_void_p), ("block_table", C.c_void_p), ("start_pos", C.c_void_p),
+        ("token_begin", C.c_void_p), ("slot_ids", C.c_void_p), ("d_k_scales", C.c_void_p), ("d_v_scales", C.c_void_p),
+        ("d_block_scales", C.c_void_p), ("k_scale", C.c_float), ("v_scale", C.c_float), ("block_table_stride", C.c_int),
+        ("num_slots", C.c_int), ("batch", C.c_int), ("num_pages", C.c_int), ("page_size", C.c_int),
+    ]
+
+
 _i32p = C.POINTER(C.c_int)
 _vp = C.c_void_p
 
@@ -110,7 +130,16 @@ SIGNATURES = {
     "pd_append_tokens_scaled": (C.c_int, [C.c_int, _vp, _vp, _vp, _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
                                           C.c_float, C.c_float, _vp, _vp, _vp]),
     "pd_paged_decode_scaled": (C.c_int, [C.c_int, C.POINTER(pd_params), C.c_int, _vp, _vp, _vp]),
+    "pd_paged_decode_block_scaled": (C.c_int, [C.c_int, C.POINTER(pd_params), C.c_int, _vp, _vp]),
     "pd_cache_set_head_scales": (C.c_int, [_vp, _vp, _vp]),
+    "pd_rope_create": (C.c_int, [C.c_int, C.POINTER(C.c_double), _i32p, C.c_int, C.c_float, C.POINTER(_vp)]),
+    "pd_rope_destroy": (None, [_vp]),
+    "pd_qk_norm_rope": (C.c_int, [C.POINTER(pd_qkv), _vp, _vp, C.c_longlong, _vp, C.c_longlong, _vp]),
+    "pd_scale_block_tokens": (C.c_int, [C.c_int]),
+    "pd_append_qkv": (C.c_int, [C.c_int, C.POINTER(pd_qkv), _vp, C.POINTER(pd_append_target), _vp, _vp]),
+    "pd_cache_append_qkv": (C.c_int, [_vp, C.c_int, _i32p, _i32p, C.POINTER(pd_qkv), _vp, _vp, _vp]),
+    "pd_cache_set_block_scales": (C.c_int, [_vp, C.c_int]),
+    "pd_cache_block_scales": (_vp, [_vp]),
     "pd_cache_bytes_per_page": (C.c_size_t, [C.POINTER(pd_cache_config)]),
     "pd_cache_pages_for_budget": (C.c_int, [C.POINTER(pd_cache_config), C.c_size_t]),
     "pd_cache_create": (C.c_int, [C.POINTER(pd_cache_config), C.POINTER(_vp)]),

@@ -31,6 +31,7 @@
 //    the merge kernel, launched as a programmatic dependent, handles rows cut in many pieces.
 //  * Optional extras behind null pointers: per-kv-head scales, outputs stored into the gathered buffers
 //    of peer GPUs, a per-CTA record of busy time and tiles for the host's adaptive cut.
+//  * BS = true (e4m3 cache): one scale per (block of at most 16 tokens, kv head) for K and for V, see BlockScales.
 
 #include <cuda.h>
 #include <cuda_fp16.h>
@@ -75,6 +76,16 @@ constexpr unsigned ST_WORKSPACE      = 6;  // the plan has more segments than th
 struct HeadScales {
     const float* k;
     const float* v;
+};
+
+// Scales of a block-scaled e4m3 cache: float pairs (K, V) at [page][kv head][block of the page]; a block is the largest
+// power of two of tokens that divides the page size, at most 16.  The producer warp brings a tile's pairs into the
+// tile's stage with 8-byte asynchronous copies that arrive on the same barrier as the tile: 8 bytes beside 4 KB of K and V per
+// 16 tokens and head.
+struct BlockScales {
+    const float2* scales;
+    int log2_block;
+    int num_pages;      // pairs of pages outside [0, num_pages) are not read
 };
 
 // Optional per-CTA record for the host's adaptive cut: every launch adds the CTA's busy nanoseconds to
@@ -158,6 +169,10 @@ struct Shape {
     static constexpr int OUT_STAGE_BYTES  = HEADS > 1 ? C::WARPS * GROUP * HEAD_DIM * 2 : 0;
     // +1024: the pipeline is aligned to the 128B-swizzle period by hand
     static constexpr int SMEM_BYTES  = 1024 + OUT_STAGE_OFFSET + OUT_STAGE_BYTES;
+    // Block-scaled cache: (K, V) scale pairs of a stage's tile, behind everything else, [block of the tile][kv head].
+    static constexpr int SCALE_OFFSET = OUT_STAGE_OFFSET + OUT_STAGE_BYTES;
+    static __host__ __device__ constexpr int scale_slot_bytes(int log2_block) { return (TILE >> log2_block) * HEADS * 8; }
+    static __host__ __device__ constexpr int scaled_smem_bytes(int log2_block) { return SMEM_BYTES + C::STAGES * scale_slot_bytes(log2_block); }
     static_assert(sizeof(KV) == 2 ? (HEADS == 1 || C::GROUPS_PER_WARP == 1) : C::GROUPS_PER_WARP % 2 == 0,
                   "a warp works on 16-token units of an fp16 cache, 32-token units of an e4m3 cache");
     static_assert(GROUP >= 1 && GROUP <= 8, "a KV group fills the 8 columns of one MMA");
@@ -226,6 +241,14 @@ __device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  :: "r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+// 8 bytes global -> shared without waiting; `live` false: nothing is read and the pair becomes zeros.
+__device__ __forceinline__ void cp_async8(uint32_t dst, const void* src, bool live) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" :: "r"(dst), "l"(src), "r"(live ? 8 : 0) : "memory");
+}
+// One arrival on `bar` once this thread's copies so far have landed.
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" :: "r"(bar) : "memory");
 }
 __device__ __forceinline__ uint32_t lds32(uint32_t addr) {
     uint32_t v;
@@ -417,11 +440,17 @@ __device__ __forceinline__ void ldmatrix_b8_x2_trans(uint32_t (&r)[4], uint32_t 
 }
 
 // grp_row: first token of the group inside the tile; grp_valid (1..32+): how many of its tokens exist.
-template<typename Rows>
+//
+// BS: scale_of(t) gives token t's (K scale, V scale) and `qk_scale` is without a K scale.  The V scale joins the softmax
+// as an exponent: y = x + log2(vs) takes x's place in the running maximum and the weights w = 2^(y - m), which
+// therefore stay in [0, 1] with the largest at 1 whatever the scales are (w is rounded to fp16 for the PV
+// product; a plain p * vs would lose bits to fp16's subnormals), and the denominator takes w / vs back out in fp32:
+//   out = sum_t w_t V_t / sum_t w_t / vs_t.   m + log2(sum) is still the log-sum-exp of x, so split rows merge as ever.
+template<bool BS, typename Rows, typename Scales>
 __device__ __forceinline__ bool process_group_e4m3(const uint32_t k_tile, const uint32_t v_tile, const Rows rows,
                                                    const int grp_row, const int grp_valid, const uint32_t (&qb)[8][2],
                                                    float (&acc)[8][4], float (&m_run)[2], float (&l_run)[2],
-                                                   const float qk_scale, const int lane)
+                                                   const float qk_scale, const int lane, const Scales scale_of)
 {
     const int g = lane >> 2, qd = lane & 3;
     bool wrote = false;
@@ -438,6 +467,7 @@ __device__ __forceinline__ bool process_group_e4m3(const uint32_t k_tile, const 
     // ---- 1. S^T = K Q^T for both 16-token halves, two interleaved accumulators each.
     const int tok_lo = g, tok_hi = tau16(g + 8);      // tokens of MMA rows g, g + 8 within a half
     float x[2][4];
+    float inv_vs[2][2] = {{1.f, 1.f}, {1.f, 1.f}};    // BS: per half and token (lo, hi)
 #pragma unroll
     for (int hh = 0; hh < 2; hh++) {
         const uint32_t r0 = rows(grp_row + 16 * hh + tok_lo, 0), r1 = rows(grp_row + 16 * hh + tok_hi, 0);
@@ -455,8 +485,15 @@ __device__ __forceinline__ bool process_group_e4m3(const uint32_t k_tile, const 
                 else       mma_16816(s0, a, qb[ks][0], qb[ks][1]);
             }
         }
+        if constexpr (BS) {
+            float ks[2], log_vs[2];
+            scale_of(grp_row + 16 * hh, 16 * hh, tok_lo, tok_hi, grp_valid, ks, log_vs, inv_vs[hh]);
 #pragma unroll
-        for (int i = 0; i < 4; i++) x[hh][i] = (s0[i] + s1[i]) * qk_scale;
+            for (int i = 0; i < 4; i++) x[hh][i] = fmaf(s0[i] + s1[i], qk_scale * ks[i >> 1], log_vs[i >> 1]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[hh][i] = (s0[i] + s1[i]) * qk_scale;
+        }
         if (grp_valid < 32) {
             if (16 * hh + tok_lo >= grp_valid) { x[hh][0] = -INFINITY; x[hh][1] = -INFINITY; }
             if (16 * hh + tok_hi >= grp_valid) { x[hh][2] = -INFINITY; x[hh][3] = -INFINITY; }
@@ -483,8 +520,19 @@ __device__ __forceinline__ bool process_group_e4m3(const uint32_t k_tile, const 
     for (int hh = 0; hh < 2; hh++)
 #pragma unroll
         for (int i = 0; i < 4; i++) pr[hh][i] = exp2f(x[hh][i] - m_run[i & 1]);
-    l_run[0] = l_run[0] * alpha[0] + ((pr[0][0] + pr[0][2]) + (pr[1][0] + pr[1][2]));
-    l_run[1] = l_run[1] * alpha[1] + ((pr[0][1] + pr[0][3]) + (pr[1][1] + pr[1][3]));
+    if constexpr (BS) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            float sum = pr[0][h] * inv_vs[0][0];
+            sum = fmaf(pr[0][2 + h], inv_vs[0][1], sum);
+            sum = fmaf(pr[1][h], inv_vs[1][0], sum);
+            sum = fmaf(pr[1][2 + h], inv_vs[1][1], sum);
+            l_run[h] = l_run[h] * alpha[h] + sum;
+        }
+    } else {
+        l_run[0] = l_run[0] * alpha[0] + ((pr[0][0] + pr[0][2]) + (pr[1][0] + pr[1][2]));
+        l_run[1] = l_run[1] * alpha[1] + ((pr[0][1] + pr[0][3]) + (pr[1][1] + pr[1][3]));
+    }
     // the accumulators only change scale when some maximum moved, which after the first tiles is rare
     if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
 #pragma unroll
@@ -612,14 +660,15 @@ __device__ __forceinline__ void merge_item(const pd_params& p, const GatherOut& 
 
 // ---- decode kernel ---------------------------------------------------------------
 
-template<typename KV, int GROUP, typename C>
+template<typename KV, int GROUP, typename C, bool BS = false>
 __global__ void __launch_bounds__((C::WARPS + 1) * 32, C::MIN_CTAS)
 paged_decode_kernel(const __grid_constant__ pd_params p, const __grid_constant__ CUtensorMap k_map,
                     const __grid_constant__ CUtensorMap v_map, const int btl /* log2(tokens per box) */,
                     const int row_gather /* boxes are four rows gathered one by one: the maps are 2-D [pool row][dims] */,
                     const int seg_limit /* segments the split-row workspace holds; 0 = sized by the plan's owner */,
                     unsigned* __restrict__ status, const __grid_constant__ GatherOut gp,
-                    const __grid_constant__ HeadScales hs, const __grid_constant__ CtaStats st)
+                    const __grid_constant__ HeadScales hs, const __grid_constant__ CtaStats st,
+                    const __grid_constant__ BlockScales bs)
 {
     const unsigned long long t_entry = (st.slots && threadIdx.x == 0) ? global_ns() : 0ull;
 #ifdef PD_B200_LOAD_ONLY
@@ -667,7 +716,7 @@ paged_decode_kernel(const __grid_constant__ pd_params p, const __grid_constant__
         asm volatile("prefetch.tensormap [%0];" :: "l"(&v_map) : "memory");
     }
     if (tid == 0) {
-        for (int s = 0; s < STAGES; s++) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), C::WARPS); }
+        for (int s = 0; s < STAGES; s++) { mbar_init(full_bar(s), BS ? 33 : 1); mbar_init(empty_bar(s), C::WARPS); }
         mbar_init(sync_bar, C::WARPS);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -752,6 +801,25 @@ paged_decode_kernel(const __grid_constant__ pd_params p, const __grid_constant__
                 for (int j = lane; j < nb; j += 32)
                     copy_box(j, make_int4(__ldg(bt + (tile_tok + (j << btl)) / ps), 0, 0, 0));
             }
+            if constexpr (BS) {
+                // the tile's scale pairs, one per lane and round; a block never straddles a box
+                static_assert(FP8, "block scales belong to the e4m3 cache");
+                const int pairs = ((valid + (1 << bs.log2_block) - 1) >> bs.log2_block) * S::HEADS;
+                const int per_page = ps >> bs.log2_block;
+                const uint32_t slot = pipe + S::SCALE_OFFSET + stage * S::scale_slot_bytes(bs.log2_block);
+                for (int e0 = 0; e0 < pairs; e0 += 32) {
+                    const int e = min(e0 + lane, pairs - 1);
+                    const int t = e / S::HEADS << bs.log2_block;     // first token of the block, within the tile
+                    const int head = S::HEADS == 1 ? sg.y : e % S::HEADS;
+                    int pg = __shfl_sync(0xffffffffu, my_page.x, lane0 + (t >> btl));
+                    if (S::HEADS == 1 && row_gather) pg = __ldg(bt + (tile_tok + t) / ps);   // several pages to a box
+                    const bool live = pg >= 0 && pg < bs.num_pages;
+                    const float2* src = bs.scales + (static_cast<size_t>(live ? pg : 0) * p.num_kv_heads + head) * per_page
+                                        + ((tile_tok + t) % ps >> bs.log2_block);
+                    if (e0 + lane < pairs) cp_async8(slot + e * 8, src, live);
+                }
+                cp_async_arrive(full_bar(stage));
+            }
             issued++;
             if (++p_stage == nst) { p_stage = 0; p_phase ^= 1; }
             return true;
@@ -816,7 +884,8 @@ paged_decode_kernel(const __grid_constant__ pd_params p, const __grid_constant__
     // softmax runs in base 2; with per-head scales the factor belongs to the segment's kv head
     float qk_scale = p.sm_scale * p.k_scale * 1.4426950408889634f;
     float v_scale  = p.v_scale;
-    if constexpr (S::HEADS > 1) {
+    if constexpr (BS) { qk_scale = p.sm_scale * 1.4426950408889634f; v_scale = 1.f; }
+    if constexpr (S::HEADS > 1 && !BS) {
         if (hs.k) qk_scale = p.sm_scale * __ldg(hs.k + warp) * 1.4426950408889634f;
         if (hs.v) v_scale = __ldg(hs.v + warp);
     }
@@ -844,7 +913,7 @@ paged_decode_kernel(const __grid_constant__ pd_params p, const __grid_constant__
     for (int seg = seg_begin; alive && seg < seg_end; seg++) {
         const int4 sg = __ldg(segments + seg);
         bool need_q = true;   // Q^T fragments are read from the slot of the segment's first tile
-        if constexpr (S::HEADS == 1) {
+        if constexpr (S::HEADS == 1 && !BS) {
             if (hs.k) qk_scale = p.sm_scale * __ldg(hs.k + sg.y) * 1.4426950408889634f;
             if (hs.v) v_scale = __ldg(hs.v + sg.y);
         }
@@ -912,8 +981,28 @@ paged_decode_kernel(const __grid_constant__ pd_params p, const __grid_constant__
                 const int grp_valid = valid - grp_row;            // >= 1; short only in a sequence's last group
                 const int box_head = S::HEADS > 1 ? warp : 0;
                 auto rows = [&](int t, int panel) { return row_offset<KV, S::HEADS>(t, panel, btl, box_head); };
-                if constexpr (FP8)
-                    wrote |= process_group_e4m3(k_tile, v_tile, rows, grp_row, grp_valid, qb, acc, m_run, l_run, qk_scale, lane);
+                if constexpr (FP8) {
+                    // (K scale, log2 and reciprocal of the V scale) of the lane's two tokens of a 16-token half; tokens that
+                    // do not exist, and blocks nothing was ever written to (zeros), count as scale 1
+                    const uint32_t slot = pipe + S::SCALE_OFFSET + stage * S::scale_slot_bytes(bs.log2_block);
+                    auto scale_of = [&](int t0, int first, int lo, int hi, int live, float (&ks)[2], float (&log_vs)[2], float (&inv)[2]) {
+#pragma unroll
+                        for (int i = 0; i < 2; i++) {
+                            if (i == 1 && bs.log2_block == 4) { ks[1] = ks[0]; log_vs[1] = log_vs[0]; inv[1] = inv[0]; break; }
+                            const int in_half = bs.log2_block == 4 ? 0 : i ? hi : lo;
+                            float2 kv = make_float2(1.f, 1.f);
+                            if (first + in_half < live) {
+                                const uint2 raw = lds64(slot + (((t0 + in_half) >> bs.log2_block) * S::HEADS + box_head) * 8);
+                                kv = make_float2(__uint_as_float(raw.x), __uint_as_float(raw.y));
+                                if (!(kv.y > 0.f)) kv.y = 1.f;
+                            }
+                            ks[i] = kv.x;
+                            log_vs[i] = __log2f(kv.y);
+                            inv[i] = __fdividef(1.f, kv.y);
+                        }
+                    };
+                    wrote |= process_group_e4m3<BS>(k_tile, v_tile, rows, grp_row, grp_valid, qb, acc, m_run, l_run, qk_scale, lane, scale_of);
+                }
                 else
                     wrote |= process_group_f16(k_tile, v_tile, rows, grp_row, grp_valid, qb, acc, m_run, l_run, qk_scale, lane);
             }

@@ -10,6 +10,7 @@
 #include "decode_kernel.cuh"
 #include "plan_kernel.cuh"
 #include "probe_kernel.cuh"
+#include "rows_kernel.cuh"
 
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -21,6 +22,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
+#include <new>
 #include <numeric>
 #include <random>
 #include <string>
@@ -73,16 +75,31 @@ struct KernelInfo {
     const void* fn;
     int tile, threads, smem, per_sm, stages;
     void (*launch)(const pd_params&, const CUtensorMap&, const CUtensorMap&, int, int, int, unsigned*, const pdk::GatherOut&,
-                   const pdk::HeadScales&, const pdk::CtaStats&, cudaStream_t);
+                   const pdk::HeadScales&, const pdk::CtaStats&, const pdk::BlockScales&, cudaStream_t);
     void (*merge)(const pd_params&, int, cudaStream_t);
+    // the same shape over a block-scaled cache (e4m3 only): launched where BlockScales carries an array
+    const void* scaled_fn;
+    int scaled_smem;               // with one scale per token, the most it can need
 };
 
 template<typename KV, int GROUP, typename C>
 void launch_decode(const pd_params& p, const CUtensorMap& km, const CUtensorMap& vm, int btl, int row_gather, int seg_limit,
                    unsigned* status, const pdk::GatherOut& gather, const pdk::HeadScales& scales, const pdk::CtaStats& stats,
-                   cudaStream_t stream) {
+                   const pdk::BlockScales& blocks, cudaStream_t stream) {
     using S = pdk::Shape<KV, GROUP, C>;
-    pdk::paged_decode_kernel<KV, GROUP, C><<<p.num_ctas, S::THREADS, S::SMEM_BYTES, stream>>>(p, km, vm, btl, row_gather, seg_limit, status, gather, scales, stats);
+    if constexpr (sizeof(KV) == 1) {
+        if (blocks.scales) {
+            pdk::paged_decode_kernel<KV, GROUP, C, true><<<p.num_ctas, S::THREADS, S::scaled_smem_bytes(blocks.log2_block), stream>>>(
+                p, km, vm, btl, row_gather, seg_limit, status, gather, scales, stats, blocks);
+            return;
+        }
+    }
+    pdk::paged_decode_kernel<KV, GROUP, C><<<p.num_ctas, S::THREADS, S::SMEM_BYTES, stream>>>(p, km, vm, btl, row_gather, seg_limit, status, gather, scales, stats, blocks);
+}
+template<typename KV, int GROUP, typename C>
+const void* scaled_kernel() {
+    if constexpr (sizeof(KV) == 1) return reinterpret_cast<const void*>(&pdk::paged_decode_kernel<KV, GROUP, C, true>);
+    else return nullptr;
 }
 // The merge kernel is launched as a programmatic dependent of the decode kernel before it: its CTAs are
 // placed while the decode grid drains and wait inside the kernel (griddepcontrol.wait) until that grid is
@@ -113,7 +130,8 @@ KernelInfo make_info() {
     using C = typename DefaultConfig<KV>::type;
     using S = pdk::Shape<KV, GROUP, C>;
     return KernelInfo{reinterpret_cast<const void*>(&pdk::paged_decode_kernel<KV, GROUP, C>), S::TILE, S::THREADS,
-                      S::SMEM_BYTES, C::MIN_CTAS, C::STAGES, &launch_decode<KV, GROUP, C>, &launch_merge<GROUP>};
+                      S::SMEM_BYTES, C::MIN_CTAS, C::STAGES, &launch_decode<KV, GROUP, C>, &launch_merge<GROUP>,
+                      scaled_kernel<KV, GROUP, C>(), S::scaled_smem_bytes(0)};
 }
 
 template<typename KV>
@@ -151,7 +169,8 @@ KernelInfo make_fused_info() {
     using C = typename FusedConfig<KV>::type;
     using S = pdk::Shape<KV, GROUP, C>;
     return KernelInfo{reinterpret_cast<const void*>(&pdk::paged_decode_kernel<KV, GROUP, C>), S::TILE, S::THREADS,
-                      S::SMEM_BYTES, C::MIN_CTAS, C::STAGES, &launch_decode<KV, GROUP, C>, &launch_merge_rows<GROUP>};
+                      S::SMEM_BYTES, C::MIN_CTAS, C::STAGES, &launch_decode<KV, GROUP, C>, &launch_merge_rows<GROUP>,
+                      scaled_kernel<KV, GROUP, C>(), S::scaled_smem_bytes(0)};
 }
 
 template<typename KV>
@@ -199,6 +218,7 @@ int configure(const KernelInfo* k) {
     std::lock_guard<std::mutex> lock(g_cfg_mutex);
     for (auto& c : g_configured) if (c.first == k->fn && c.second == dev) return PD_OK;
     PD_CUDA(cudaFuncSetAttribute(k->fn, cudaFuncAttributeMaxDynamicSharedMemorySize, k->smem));
+    if (k->scaled_fn) PD_CUDA(cudaFuncSetAttribute(k->scaled_fn, cudaFuncAttributeMaxDynamicSharedMemorySize, k->scaled_smem));
     g_configured.emplace_back(k->fn, dev);
     return PD_OK;
 }
@@ -291,6 +311,7 @@ int make_tensor_map(CUtensorMap* map, int dtype, const void* pool, int num_pages
 
 }  // namespace
 #include "host_plan.hpp"
+#include "rows_host.hpp"
 
 // ---- DevicePlan ---------------------------------------------------------------------------------
 
@@ -358,6 +379,7 @@ struct pd_cache {
     int plan_batch = 0, plan_num_q_heads = 0;
     bool plan_identity = false;
     float* d_head_scales = nullptr;       // optional per-kv-head scales: k[num_kv_heads] then v[num_kv_heads]
+    float* d_block_scales = nullptr;      // optional scales per (page, kv head, block of the page): K, V
     bool plan_on_device = false;          // the current plan was cut by pd_cache_plan_device
     const int* plan_slot_ids = nullptr;   // ... for these rows (device pointer of the caller, or null)
     std::vector<int> free_pages;
@@ -1061,7 +1083,8 @@ Selection select_schedule(int dtype, const pd_params* p, const KernelInfo* k, bo
 }
 
 int decode_impl(int dtype, const pd_params* p, int num_pages, const pdk::GatherOut& gather, void* stream_,
-                const pdk::HeadScales& scales = pdk::HeadScales{nullptr, nullptr}) {
+                const pdk::HeadScales& scales = pdk::HeadScales{nullptr, nullptr},
+                const float* block_scales = nullptr) {
     if (!p) return set_error(PD_INVALID_ARGUMENT, "paged_decode: null params");
     if (p->num_kv_heads <= 0 || p->num_q_heads % p->num_kv_heads != 0)
         return set_error(PD_INVALID_ARGUMENT, "num_q_heads must be a multiple of num_kv_heads");
@@ -1099,7 +1122,8 @@ int decode_impl(int dtype, const pd_params* p, int num_pages, const pdk::GatherO
     if (int rc = make_tensor_map(&v_map, dtype, p->v_cache, num_pages, p->num_kv_heads, p->page_size, btl, box_heads, row_gather)) return rc;
 
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-    k->launch(*p, k_map, v_map, btl, row_gather ? 1 : 0, 0, status, gather, scales, pdk::CtaStats{stats_slots}, stream);
+    const pdk::BlockScales blocks{reinterpret_cast<const float2*>(block_scales), scale_block_log2(p->page_size), num_pages};
+    k->launch(*p, k_map, v_map, btl, row_gather ? 1 : 0, 0, status, gather, scales, pdk::CtaStats{stats_slots}, blocks, stream);
     PD_CUDA(cudaGetLastError());
     if (p->needs_merge && p->needs_merge != pdk::MERGE_IN_KERNEL) {
         k->merge(*p, 0, stream);
@@ -1122,6 +1146,14 @@ int pd_paged_decode(int dtype, const pd_params* p, void* stream) {
 int pd_paged_decode_scaled(int dtype, const pd_params* p, int num_pages, const float* d_k_scales, const float* d_v_scales,
                            void* stream) {
     return decode_impl(dtype, p, num_pages, pdk::GatherOut{}, stream, pdk::HeadScales{d_k_scales, d_v_scales});
+}
+
+int pd_paged_decode_block_scaled(int dtype, const pd_params* p, int num_pages, const float* d_block_scales, void* stream) {
+    if (dtype != PD_FP8_E4M3) return set_error(PD_INVALID_ARGUMENT, "paged_decode_block_scaled: only an fp8 cache has block scales");
+    if (!d_block_scales || reinterpret_cast<uintptr_t>(d_block_scales) % 8 != 0)
+        return set_error(PD_INVALID_ARGUMENT, "paged_decode_block_scaled: block scales must be a non-null, 8-byte aligned device array");
+    if (num_pages <= 0) return set_error(PD_INVALID_ARGUMENT, "paged_decode_block_scaled: num_pages must be positive");
+    return decode_impl(dtype, p, num_pages, pdk::GatherOut{}, stream, pdk::HeadScales{nullptr, nullptr}, d_block_scales);
 }
 
 int pd_describe_launch(int dtype, const pd_params* p, int* out) {
@@ -1241,7 +1273,7 @@ int pd_paged_decode_static(int dtype, const pd_params* p, int num_segments, int 
     // whose segments lie beyond it stores nothing and reports ST_WORKSPACE instead of writing past the array.
     const int seg_limit = std::max(num_segments, 1);
     k->launch(local, k_map, v_map, btl, row_gather ? 1 : 0, seg_limit, d_status ? d_status : scratch->status, pdk::GatherOut{},
-              pdk::HeadScales{nullptr, nullptr}, pdk::CtaStats{nullptr}, stream);
+              pdk::HeadScales{nullptr, nullptr}, pdk::CtaStats{nullptr}, pdk::BlockScales{nullptr, 0, 0}, stream);
     PD_CUDA(cudaGetLastError());
     if (local.needs_merge) {
         k->merge(local, seg_limit, stream);
@@ -1260,6 +1292,9 @@ int pd_kernel_status(void* stream, unsigned* out) {
         PD_CUDA(cudaMemset(status, 0, sizeof(unsigned)));
         if ((*out >> 24) == pdk::ST_WORKSPACE)
             return set_error(PD_KERNEL_TIMEOUT, "decode kernel: the plan has more segments than the workspace holds (CTA %u gave up)",
+                             *out & 0xffffffu);
+        if ((*out >> 24) == pdk::ST_APPEND_RANGE)
+            return set_error(PD_KERNEL_TIMEOUT, "append: row %u has no place in the block table or the pool and was not stored",
                              *out & 0xffffffu);
         return set_error(PD_KERNEL_TIMEOUT, "decode kernel: bounded wait %u expired in CTA %u", *out >> 24, *out & 0xffffffu);
     }
@@ -1500,6 +1535,7 @@ void pd_cache_destroy(pd_cache* c) {
     cudaFree(c->d_seq_lens);
     cudaFree(c->d_slot_ids);
     cudaFree(c->d_head_scales);
+    cudaFree(c->d_block_scales);
     if (c->batch_staged) { cudaEventSynchronize(c->batch_staged); cudaEventDestroy(c->batch_staged); }
     if (c->batch_done) { cudaEventSynchronize(c->batch_done); cudaEventDestroy(c->batch_done); }
     cudaFreeHost(c->batch_staging);
@@ -1560,6 +1596,42 @@ int pd_cache_admit(pd_cache* c) {
     return -1;
 }
 
+}  // extern "C"
+namespace {
+// The cache as the target of an append; the caller adds which sequences.
+int cache_pages(pd_cache* c, pdk::PageArgs* t) {
+    *t = pdk::PageArgs{};
+    t->k_cache = c->d_k; t->v_cache = c->d_v;
+    t->block_table = c->d_block_table;
+    t->table_stride = c->cfg.max_pages_per_slot; t->num_slots = c->cfg.max_slots;
+    t->num_pages = c->cfg.num_pages; t->page_size = c->cfg.page_size;
+    if (c->cfg.dtype == PD_FP8_E4M3) {
+        t->inv_k = 1.f / c->cfg.k_scale; t->inv_v = 1.f / c->cfg.v_scale;
+        t->k_head_scales = c->d_head_scales;
+        t->v_head_scales = c->d_head_scales ? c->d_head_scales + c->cfg.num_kv_heads : nullptr;
+        t->block_scales = c->d_block_scales;
+    }
+    return status_word(&t->status);
+}
+// Rows into the cache's pages; x has been checked against the cache, but for its pointers where it has them.
+int cache_append_rows(pd_cache* c, const pd_qkv& x, const pd_rope* rope, const pdk::PageArgs& t, void* q_out, cudaStream_t stream) {
+    pdk::RowArgs a;
+    pdk::RopeArgs r;
+    if (int rc = fill_rows("append", &x, rope, true, &a, &r)) return rc;
+    if (int rc = check_rows("append", "q", a.q, &a.q_stride, a.hq)) return rc;
+    if (t.k_src) {
+        a.k_stride = a.v_stride = static_cast<long long>(a.hkv) * 128;
+    } else {
+        if (int rc = check_rows("append", "k", a.k, &a.k_stride, a.hkv)) return rc;
+        if (int rc = check_rows("append", "v", a.v, &a.v_stride, a.hkv)) return rc;
+    }
+    if (int rc = check_rows("append", "q_out", q_out, &a.q_out_stride, a.hq)) return rc;
+    a.q_out = q_out;
+    return launch_append(c->cfg.dtype, x.act_dtype, a, r, t, stream);
+}
+}  // namespace
+extern "C" {
+
 int pd_cache_append(pd_cache* c, int slot, const void* d_k, const void* d_v, int n, void* stream_) {
     if (!c || slot < 0 || slot >= c->cfg.max_slots || !c->occupied[slot])
         return set_error(PD_INVALID_ARGUMENT, "append: slot is not admitted");
@@ -1570,6 +1642,8 @@ int pd_cache_append(pd_cache* c, int slot, const void* d_k, const void* d_v, int
     const int new_len = old_len + n;
     const int have = static_cast<int>(c->tables[slot].size());
     const int need = (new_len + ps - 1) / ps;
+    if (c->d_block_scales && (!d_k || !d_v || unaligned16(d_k) || unaligned16(d_v)))
+        return set_error(PD_INVALID_ARGUMENT, "append: K/V buffers must be non-null and 16-byte aligned");
     if (need > c->cfg.max_pages_per_slot) return set_error(PD_LENGTH_ERROR, "append: sequence exceeds max_pages_per_slot");
     if (need - have > static_cast<int>(c->free_pages.size()))
         return set_error(PD_OUT_OF_PAGES, "append: out of pages");
@@ -1584,7 +1658,18 @@ int pd_cache_append(pd_cache* c, int slot, const void* d_k, const void* d_v, int
                                 cudaMemcpyHostToDevice, stream));
     c->seq_lens[slot] = new_len;
     PD_CUDA(cudaMemcpyAsync(c->d_seq_lens + slot, &c->seq_lens[slot], sizeof(int), cudaMemcpyHostToDevice, stream));
-    if (int rc = pd_append_tokens_scaled(c->cfg.dtype, d_k, d_v, c->d_k, c->d_v, row, old_len, n, c->cfg.num_kv_heads,
+    if (c->d_block_scales) {
+        pd_qkv x{};
+        x.k = d_k; x.v = d_v;
+        x.num_tokens = n; x.num_kv_heads = c->cfg.num_kv_heads; x.head_dim = c->cfg.head_dim;
+        pdk::PageArgs t;
+        if (int rc = cache_pages(c, &t)) return rc;
+        t.first_pos = old_len;
+        t.one_sequence = 1;
+        t.batch = 1;
+        t.block_table = row;
+        if (int rc = cache_append_rows(c, x, nullptr, t, nullptr, stream)) return rc;
+    } else if (int rc = pd_append_tokens_scaled(c->cfg.dtype, d_k, d_v, c->d_k, c->d_v, row, old_len, n, c->cfg.num_kv_heads,
                                          c->cfg.head_dim, ps, c->cfg.k_scale, c->cfg.v_scale, c->d_head_scales,
                                          c->d_head_scales ? c->d_head_scales + c->cfg.num_kv_heads : nullptr, stream))
         return rc;
@@ -1593,6 +1678,8 @@ int pd_cache_append(pd_cache* c, int slot, const void* d_k, const void* d_v, int
     return PD_OK;
 }
 
+}  // extern "C"
+namespace {
 // One decode step's appends for many slots: the allocator runs for every slot in the order given
 // (so block tables come out exactly as from the same pd_cache_append calls in that order), then
 // ONE packed host->device copy carries the job list, the new block-table entries and the new
@@ -1600,15 +1687,14 @@ int pd_cache_append(pd_cache* c, int slot, const void* d_k, const void* d_v, int
 // slots at once.  All-or-nothing: if the pool cannot hold every slot's tokens nothing changes.
 // Stream-ordered: returns without waiting; the K/V sources must stay valid until the stream
 // has run the scatter.
-int pd_cache_append_batch(pd_cache* c, int count, const int* slots, const void* const* d_k, const void* const* d_v,
-                          const int* n, void* stream_) {
-    if (!c || count < 0 || (count > 0 && (!slots || !d_k || !d_v || !n)))
-        return set_error(PD_INVALID_ARGUMENT, "append_batch: bad argument");
-    if (count == 0) return PD_OK;
-    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+// Sources are d_k / d_v per slot, or (x) the rows of one projection in the order of the slots.  Rows of x, and every
+// append into a block-scaled cache, go through the rows kernel, whose job list is (first row, start, slot) per slot.
+int append_batch_impl(pd_cache* c, int count, const int* slots, const void* const* d_k, const void* const* d_v,
+                      const int* n, const pd_qkv* x, const pd_rope* rope, void* q_out, cudaStream_t stream) {
+    const bool as_rows = x || c->d_block_scales;
     const int ps = c->cfg.page_size;
     // ---- validate everything before touching the allocator
-    long long new_pages = 0, total_units = 0;
+    long long new_pages = 0, total_units = 0, total_tokens = 0;
     std::vector<char> seen(c->cfg.max_slots, 0);
     for (int i = 0; i < count; i++) {
         const int slot = slots[i];
@@ -1618,24 +1704,31 @@ int pd_cache_append_batch(pd_cache* c, int count, const int* slots, const void* 
         seen[slot] = 1;
         if (n[i] < 0) return set_error(PD_INVALID_ARGUMENT, "append_batch: negative token count");
         if (n[i] == 0) continue;
-        if (!d_k[i] || !d_v[i] || (reinterpret_cast<uintptr_t>(d_k[i]) | reinterpret_cast<uintptr_t>(d_v[i])) % 16 != 0)
+        if (!x && (!d_k[i] || !d_v[i] || (reinterpret_cast<uintptr_t>(d_k[i]) | reinterpret_cast<uintptr_t>(d_v[i])) % 16 != 0))
             return set_error(PD_INVALID_ARGUMENT, "append_batch: K/V sources must be non-null and 16-byte aligned");
+        if (n[i] > 0x7fffffff - c->seq_lens[slot] - ps) return set_error(PD_LENGTH_ERROR, "append: sequence exceeds max_pages_per_slot");
         const int need = (c->seq_lens[slot] + n[i] + ps - 1) / ps;
         if (need > c->cfg.max_pages_per_slot) return set_error(PD_LENGTH_ERROR, "append: sequence exceeds max_pages_per_slot");
         new_pages += need - static_cast<int>(c->tables[slot].size());
         total_units += static_cast<long long>(n[i]) * c->cfg.num_kv_heads * 16;
+        total_tokens += n[i];
     }
-    if (total_units > 0x7fffffffLL) return set_error(PD_LENGTH_ERROR, "append_batch: too many tokens in one batch");
+    if (as_rows ? total_tokens > 0x7fffffffLL : total_units > 0x7fffffffLL)
+        return set_error(PD_LENGTH_ERROR, "append_batch: too many tokens in one batch");
+    if (x && total_tokens != x->num_tokens)
+        return set_error(PD_INVALID_ARGUMENT, "append_qkv: %d rows for %lld tokens", x->num_tokens, total_tokens);
     if (new_pages > static_cast<long long>(c->free_pages.size())) return set_error(PD_OUT_OF_PAGES, "append: out of pages");
 
-    // ---- packed buffer: jobs | (slot, index, page) table updates | (slot, length) updates
+    // ---- packed buffer: jobs | (slot, index, page) table updates | (slot, length) updates | rows kernel's lists
     struct TableUpdate { int slot, index, page; };
     struct LenUpdate { int slot, len; };
-    auto round16 = [](size_t x) { return (x + 15) & ~static_cast<size_t>(15); };
-    const size_t jobs_bytes = round16(sizeof(pdk::AppendJob) * count);
+    auto round16 = [](size_t v) { return (v + 15) & ~static_cast<size_t>(15); };
+    const size_t jobs_bytes = as_rows ? 0 : round16(sizeof(pdk::AppendJob) * count);
     const size_t tab_bytes  = round16(sizeof(TableUpdate) * static_cast<size_t>(new_pages));
     const size_t len_bytes  = round16(sizeof(LenUpdate) * count);
-    const size_t total = jobs_bytes + tab_bytes + len_bytes;
+    const size_t list_bytes = as_rows ? round16(sizeof(int) * (count + 1)) : 0;            // token_begin; start_pos; slot_ids
+    const size_t src_bytes  = as_rows && !x ? round16(sizeof(void*) * static_cast<size_t>(count)) : 0;   // k_src; v_src
+    const size_t total = jobs_bytes + tab_bytes + len_bytes + 3 * list_bytes + 2 * src_bytes;
     if (!c->batch_staged) PD_CUDA(cudaEventCreateWithFlags(&c->batch_staged, cudaEventDisableTiming));
     else PD_CUDA(cudaEventSynchronize(c->batch_staged));      // the previous batch still reads the staging buffer
     if (total > c->batch_cap) {
@@ -1647,12 +1740,21 @@ int pd_cache_append_batch(pd_cache* c, int count, const int* slots, const void* 
         PD_CUDA(cudaMalloc(&c->batch_device, cap));
         c->batch_cap = cap;
     }
+    pdk::PageArgs pages;
+    if (as_rows)
+        if (int rc = cache_pages(c, &pages)) return rc;
     char* h = static_cast<char*>(c->batch_staging);
+    const size_t lists_at = jobs_bytes + tab_bytes + len_bytes, src_at = lists_at + 3 * list_bytes;
     auto* jobs = reinterpret_cast<pdk::AppendJob*>(h);
     auto* tabs = reinterpret_cast<TableUpdate*>(h + jobs_bytes);
     auto* lens = reinterpret_cast<LenUpdate*>(h + jobs_bytes + tab_bytes);
+    auto* begin = reinterpret_cast<int*>(h + lists_at);
+    auto* start = reinterpret_cast<int*>(h + lists_at + list_bytes);
+    auto* rows  = reinterpret_cast<int*>(h + lists_at + 2 * list_bytes);
+    auto* k_src = reinterpret_cast<const void**>(h + src_at);
+    auto* v_src = reinterpret_cast<const void**>(h + src_at + src_bytes);
     long long units = 0;
-    int t = 0, live = 0;
+    int t = 0, live = 0, token = 0;
     for (int i = 0; i < count; i++) {
         const int slot = slots[i];
         const int old_len = c->seq_lens[slot];
@@ -1666,12 +1768,19 @@ int pd_cache_append_batch(pd_cache* c, int count, const int* slots, const void* 
         }
         c->seq_lens[slot] = old_len + n[i];
         lens[i] = LenUpdate{slot, c->seq_lens[slot]};
+        if (as_rows) {
+            begin[i] = token; start[i] = old_len; rows[i] = slot;
+            if (!x) { k_src[i] = d_k[i]; v_src[i] = d_v[i]; }
+            token += n[i];
+            continue;
+        }
         if (n[i] == 0) continue;
         jobs[live++] = pdk::AppendJob{static_cast<const __half*>(d_k[i]), static_cast<const __half*>(d_v[i]),
                                       c->d_block_table + static_cast<size_t>(slot) * c->cfg.max_pages_per_slot,
                                       old_len, n[i], static_cast<int>(units)};
         units += static_cast<long long>(n[i]) * c->cfg.num_kv_heads * 16;
     }
+    if (as_rows) begin[count] = token;
     PD_CUDA(cudaMemcpyAsync(c->batch_device, c->batch_staging, total, cudaMemcpyHostToDevice, stream));
     PD_CUDA(cudaEventRecord(c->batch_staged, stream));
     char* d = static_cast<char*>(c->batch_device);
@@ -1679,7 +1788,21 @@ int pd_cache_append_batch(pd_cache* c, int count, const int* slots, const void* 
         reinterpret_cast<const int*>(d + jobs_bytes), t, reinterpret_cast<const int*>(d + jobs_bytes + tab_bytes), count,
         c->d_block_table, c->cfg.max_pages_per_slot, c->d_seq_lens);
     PD_CUDA(cudaGetLastError());
-    if (live > 0) {
+    if (as_rows && token > 0) {
+        pages.batch = count;
+        pages.token_begin = reinterpret_cast<const int*>(d + lists_at);
+        pages.start_pos = reinterpret_cast<const int*>(d + lists_at + list_bytes);
+        pages.slot_ids = reinterpret_cast<const int*>(d + lists_at + 2 * list_bytes);
+        pd_qkv sources{};
+        if (!x) {
+            pages.k_src = reinterpret_cast<const void* const*>(d + src_at);
+            pages.v_src = reinterpret_cast<const void* const*>(d + src_at + src_bytes);
+            sources.num_tokens = token;
+            sources.num_kv_heads = c->cfg.num_kv_heads;
+            sources.head_dim = c->cfg.head_dim;
+        }
+        if (int rc = cache_append_rows(c, x ? *x : sources, rope, pages, q_out, stream)) return rc;
+    } else if (live > 0) {
         const int blocks = static_cast<int>(std::min<long long>((units + 255) / 256, 148 * 16));
         const bool fp8 = c->cfg.dtype == PD_FP8_E4M3;
         const float ik = fp8 ? 1.f / c->cfg.k_scale : 1.f, iv = fp8 ? 1.f / c->cfg.v_scale : 1.f;
@@ -1696,6 +1819,36 @@ int pd_cache_append_batch(pd_cache* c, int count, const int* slots, const void* 
     PD_CUDA(cudaEventRecord(c->batch_done, stream));
     c->batch_pending = true;
     return PD_OK;
+}
+}  // namespace
+extern "C" {
+
+int pd_cache_append_batch(pd_cache* c, int count, const int* slots, const void* const* d_k, const void* const* d_v,
+                          const int* n, void* stream) {
+    if (!c || count < 0 || (count > 0 && (!slots || !d_k || !d_v || !n)))
+        return set_error(PD_INVALID_ARGUMENT, "append_batch: bad argument");
+    if (count == 0) return PD_OK;
+    return append_batch_impl(c, count, slots, d_k, d_v, n, nullptr, nullptr, nullptr, static_cast<cudaStream_t>(stream));
+}
+
+int pd_cache_append_qkv(pd_cache* c, int count, const int* slots, const int* n, const pd_qkv* x, const pd_rope* rope,
+                        void* q_out, void* stream) {
+    if (!c || !x || count < 0 || (count > 0 && (!slots || !n))) return set_error(PD_INVALID_ARGUMENT, "append_qkv: bad argument");
+    if (x->num_kv_heads != c->cfg.num_kv_heads) return set_error(PD_INVALID_ARGUMENT, "append_qkv: the cache has %d kv heads", c->cfg.num_kv_heads);
+    // every check of the rows before the allocator moves
+    pdk::RowArgs a;
+    pdk::RopeArgs r;
+    if (int rc = fill_rows("append_qkv", x, rope, true, &a, &r)) return rc;
+    long long out_stride = 0;
+    if (x->num_tokens > 0) {
+        if (int rc = check_rows("append_qkv", "q", a.q, &a.q_stride, a.hq)) return rc;
+        if (int rc = check_rows("append_qkv", "k", a.k, &a.k_stride, a.hkv)) return rc;
+        if (int rc = check_rows("append_qkv", "v", a.v, &a.v_stride, a.hkv)) return rc;
+        if (int rc = check_rows("append_qkv", "q_out", q_out, &out_stride, a.hq)) return rc;
+    }
+    if (count == 0)
+        return x->num_tokens == 0 ? PD_OK : set_error(PD_INVALID_ARGUMENT, "append_qkv: %d rows for 0 tokens", x->num_tokens);
+    return append_batch_impl(c, count, slots, nullptr, nullptr, n, x, rope, q_out, static_cast<cudaStream_t>(stream));
 }
 
 int pd_cache_release(pd_cache* c, int slot) {
@@ -1801,6 +1954,7 @@ int pd_cache_run(pd_cache* c, const void* d_q, void* d_out, void* stream) {
     p.batch = c->plan_batch;
     p.num_q_heads = c->plan_num_q_heads;
     pd_device_plan_bind(c->device_plan, &p);
+    if (c->d_block_scales) return pd_paged_decode_block_scaled(c->cfg.dtype, &p, c->cfg.num_pages, c->d_block_scales, stream);
     return pd_paged_decode_scaled(c->cfg.dtype, &p, c->cfg.num_pages, c->d_head_scales,
                                   c->d_head_scales ? c->d_head_scales + c->cfg.num_kv_heads : nullptr, stream);
 }
@@ -1821,6 +1975,7 @@ int pd_cache_set_head_scales(pd_cache* c, const float* k_scales, const float* v_
     if (c->cfg.dtype != PD_FP8_E4M3) return set_error(PD_INVALID_ARGUMENT, "set_head_scales: only an fp8 cache is quantised");
     if ((k_scales == nullptr) != (v_scales == nullptr))
         return set_error(PD_INVALID_ARGUMENT, "set_head_scales: give both arrays or neither");
+    if (k_scales && c->d_block_scales) return set_error(PD_INVALID_ARGUMENT, "set_head_scales: the cache has block scales");
     for (int len : c->seq_lens)
         if (len > 0) return set_error(PD_INVALID_ARGUMENT, "set_head_scales: the cache already holds tokens quantised with the old scales");
     if (!k_scales) {
@@ -1836,6 +1991,29 @@ int pd_cache_set_head_scales(pd_cache* c, const float* k_scales, const float* v_
     PD_CUDA(cudaMemcpy(c->d_head_scales + n, v_scales, sizeof(float) * n, cudaMemcpyHostToDevice));
     return PD_OK;
 }
+
+int pd_cache_set_block_scales(pd_cache* c, int on) {
+    if (!c) return set_error(PD_INVALID_ARGUMENT, "set_block_scales: null cache");
+    if (c->cfg.dtype != PD_FP8_E4M3) return set_error(PD_INVALID_ARGUMENT, "set_block_scales: only an fp8 cache is quantised");
+    for (int len : c->seq_lens)
+        if (len > 0) return set_error(PD_INVALID_ARGUMENT, "set_block_scales: the cache already holds tokens quantised with the old scales");
+    if (!on) {
+        PD_CUDA(cudaFree(c->d_block_scales));
+        c->d_block_scales = nullptr;
+        return PD_OK;
+    }
+    if (c->d_head_scales) return set_error(PD_INVALID_ARGUMENT, "set_block_scales: the cache has head scales");
+    if (c->d_block_scales) return PD_OK;
+    const size_t pairs = static_cast<size_t>(c->cfg.num_pages) * c->cfg.num_kv_heads * (c->cfg.page_size >> scale_block_log2(c->cfg.page_size));
+    float* scales = nullptr;
+    PD_CUDA(cudaMalloc(&scales, 2 * sizeof(float) * pairs));
+    const cudaError_t e = cudaMemset(scales, 0, 2 * sizeof(float) * pairs);   // 0: nothing written yet
+    if (e != cudaSuccess) { cudaFree(scales); return set_error(PD_CUDA_ERROR, "set_block_scales: %s", cudaGetErrorString(e)); }
+    c->d_block_scales = scales;
+    return PD_OK;
+}
+
+float* pd_cache_block_scales(const pd_cache* c) { return c ? c->d_block_scales : nullptr; }
 
 int pd_cache_decode(pd_cache* c, const void* d_q, void* d_out, int batch, int num_q_heads, int num_ctas, void* stream) {
     if (!c || batch < 0) return set_error(PD_INVALID_ARGUMENT, "decode: bad argument");

@@ -12,15 +12,24 @@ import enum
 import numpy as np
 
 from . import _lib
-from ._lib import InvalidArgument, LengthError, check, pd_cache_config, pd_params
+from ._lib import (InvalidArgument, LengthError, check, pd_append_target, pd_cache_config, pd_params,
+                   pd_qkv)
 
 DecodeParams = pd_params
+QKVParams = pd_qkv
+AppendTarget = pd_append_target
 
 
 class KVDtype(enum.IntEnum):
     """decode::KVDtype (src/decode/decode_types.hpp:8)."""
     FP16 = 0
     FP8_E4M3 = 1
+
+
+class ActDtype(enum.IntEnum):
+    """Type of the q, k and v rows of a model step (not in the reference, whose rows are always fp16)."""
+    FP16 = 0
+    BF16 = 1
 
 
 def kv_dtype_bytes(t):
@@ -240,10 +249,16 @@ class DevicePlan:
         return DecodePlan(h)
 
 
-def paged_decode(dtype, params, stream=0, num_pages=0, d_k_scales=None, d_v_scales=None):
+def paged_decode(dtype, params, stream=0, num_pages=0, d_k_scales=None, d_v_scales=None, d_block_scales=None):
     """decode::paged_decode (src/decode/decode.hpp:66).  d_k_scales / d_v_scales (not in the reference):
-    device arrays of one dequantisation scale per kv head, replacing params.k_scale / v_scale."""
-    if d_k_scales is None and d_v_scales is None:
+    device arrays of one dequantisation scale per kv head, replacing params.k_scale / v_scale.  d_block_scales (not
+    in the reference either): the e4m3 cache's scales per block of tokens and kv head, device floats
+    [num_pages, num_kv_heads, page_size / scale_block_tokens(page_size), 2] (K, V); needs num_pages."""
+    if d_block_scales is not None:
+        if d_k_scales is not None or d_v_scales is not None:
+            raise InvalidArgument("paged_decode: head scales and block scales exclude each other")
+        check(_lib.lib().pd_paged_decode_block_scaled(int(dtype), C.byref(params), num_pages, _ptr(d_block_scales), stream))
+    elif d_k_scales is None and d_v_scales is None:
         check(_lib.lib().pd_paged_decode_bounded(int(dtype), C.byref(params), num_pages, stream))
     else:
         check(_lib.lib().pd_paged_decode_scaled(int(dtype), C.byref(params), num_pages, _ptr(d_k_scales), _ptr(d_v_scales),
@@ -297,6 +312,173 @@ def append_tokens(dtype, d_k, d_v, k_cache, v_cache, d_block_table_row, start_po
     check(_lib.lib().pd_append_tokens_scaled(int(dtype), _ptr(d_k), _ptr(d_v), _ptr(k_cache), _ptr(v_cache),
                                              _ptr(d_block_table_row), start_pos, n, num_kv_heads, head_dim, page_size,
                                              k_scale, v_scale, _ptr(d_k_scales), _ptr(d_v_scales), stream))
+
+
+class Rope:
+    """A rotation of the first 2 * len(inv_freq) dims of every head (not in the reference).  Frequency i turns its pair
+    by position * inv_freq[i] radians; pairs are (i, i + R/2), or (2i, 2i + 1) with `interleaved`.  axes[i] names the row of
+    the positions that drives frequency i (0..3; None: one axis for all).  `scale` multiplies sine and cosine."""
+
+    def __init__(self, inv_freq, interleaved=False, axes=None, scale=1.0):
+        self._h = None
+        f = np.ascontiguousarray(inv_freq, dtype=np.float64)
+        a = None if axes is None else np.ascontiguousarray(axes, dtype=np.int32)
+        if f.ndim != 1 or (a is not None and a.shape != f.shape):
+            raise InvalidArgument("Rope: one frequency, and one axis where there are axes, per pair")
+        h = C.c_void_p()
+        check(_lib.lib().pd_rope_create(2 * len(f), f.ctypes.data_as(C.POINTER(C.c_double)),
+                                        None if a is None else a.ctypes.data_as(C.POINTER(C.c_int)), int(bool(interleaved)),
+                                        float(scale), C.byref(h)))
+        self._h = h
+
+    @classmethod
+    def with_base(cls, base=10000.0, rotary_dim=128, **kw):
+        """The usual frequencies base^(-2i / rotary_dim)."""
+        return cls(float(base) ** (-np.arange(0, rotary_dim, 2, dtype=np.float64) / rotary_dim), **kw)
+
+    def __del__(self):
+        if getattr(self, "_h", None):
+            try:
+                _lib.lib().pd_rope_destroy(self._h)
+            except Exception:      # interpreter shutdown: the module is already gone
+                pass
+            self._h = None
+
+
+def _check_device(index):
+    """The library works on the current device; tensors of another one are refused instead of faulting."""
+    if index is not None:
+        import torch
+        if torch.cuda.current_device() != index:
+            raise InvalidArgument(f"tensors on cuda:{index}, but the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _device_index(tensors):
+    found = {x.device for x in tensors if x is not None}
+    if len(found) > 1 or any(d.type != "cuda" for d in found):
+        raise InvalidArgument("tensors must be on one CUDA device, found " + ", ".join(sorted(map(str, found))))
+    return found.pop().index if found else None
+
+
+def _rows_of(name, x, dtype=None, tokens=None, heads=None):
+    """[tokens, heads, 128] tensor -> its row stride; heads of a row must be dense."""
+    if x.dim() != 3 or x.shape[2] != 128 or (x.numel() and x.stride(2) != 1) or (x.numel() and x.shape[1] > 1 and x.stride(1) != 128):
+        raise InvalidArgument(f"{name} must be [tokens, heads, 128] with dense heads")
+    if (dtype is not None and x.dtype != dtype) or (tokens is not None and x.shape[0] != tokens) or (heads is not None and x.shape[1] != heads):
+        raise InvalidArgument(f"{name} does not match the other rows")
+    return x.stride(0) if x.shape[0] > 1 else 0     # one row, or none: the stride says nothing
+
+
+def _vector(name, x, dtype, n):
+    if x is not None and (x.dtype != dtype or x.dim() != 1 or x.shape[0] != n or not x.is_contiguous()):
+        raise InvalidArgument(f"{name} must be a dense {dtype} tensor of {n} elements")
+    return _ptr(x)
+
+
+def qkv_params(q, k, v=None, q_norm=None, k_norm=None, eps=1e-6, positions=None):
+    """The rows of a call from tensors [tokens, heads, 128] (fp16 or bf16; slices of one projection are fine): q may be None.
+    q_norm, k_norm: weights [128] of the per-head RMS norm, in the rows' type; positions: int32 [tokens] or [axes, tokens].
+    The struct keeps the tensors alive and may be used for any number of calls on their current contents."""
+    import torch
+    x = QKVParams()
+    if k.dtype not in (torch.float16, torch.bfloat16):
+        raise InvalidArgument("rows must be fp16 or bf16")
+    tokens = k.shape[0]
+    x.k_stride, x.k = _rows_of("k", k), k.data_ptr()
+    if q is not None:
+        x.q_stride, x.q, x.num_q_heads = _rows_of("q", q, k.dtype, tokens), q.data_ptr(), q.shape[1]
+    if v is not None:
+        x.v_stride, x.v = _rows_of("v", v, k.dtype, tokens, k.shape[1]), v.data_ptr()
+    x.q_norm, x.k_norm = _vector("q_norm", q_norm, k.dtype, 128), _vector("k_norm", k_norm, k.dtype, 128)
+    if positions is not None:
+        p = positions if positions.dim() == 2 else positions.unsqueeze(0)
+        if p.dtype != torch.int32 or p.dim() != 2 or p.shape[1] != tokens or (tokens > 1 and p.stride(1) != 1):
+            raise InvalidArgument("positions must be int32 [tokens] or [axes, tokens], dense along the tokens")
+        if p.shape[0] > 1 and p.stride(0) < tokens:
+            p = p.contiguous()      # a broadcast axis
+        x.positions, x.num_axes, x.positions_stride = p.data_ptr(), p.shape[0], p.stride(0) if p.shape[0] > 1 else tokens
+        positions = p
+    x.act_dtype = ActDtype.FP16 if k.dtype == torch.float16 else ActDtype.BF16
+    x.num_tokens, x.num_kv_heads, x.head_dim, x.eps = tokens, k.shape[1], 128, eps
+    x._keep = (q, k, v, q_norm, k_norm, positions)
+    x._device = _device_index(x._keep)
+    return x
+
+
+def qk_norm_rope(x, rope, d_q_out, d_k_out, stream=0):
+    """Per-head RMS norm (where x has weights) and rotation (rope may be None) of the q and k rows in one pass (not in the
+    reference).  Outputs like the inputs: tensors [tokens, heads, 128] (the inputs themselves: in place), or pointers
+    to dense rows."""
+    _check_device(getattr(x, "_device", None))
+    strides = []
+    for name, out, heads in (("q_out", d_q_out, x.num_q_heads), ("k_out", d_k_out, x.num_kv_heads)):
+        strides.append(_rows_of(name, out, x._keep[1].dtype, x.num_tokens, heads) if hasattr(out, "dim") and hasattr(x, "_keep") else 0)
+    check(_lib.lib().pd_qk_norm_rope(C.byref(x), rope._h if rope is not None else None, _ptr(d_q_out), strides[0],
+                                     _ptr(d_k_out), strides[1], stream))
+
+
+def scale_block_tokens(page_size):
+    """Tokens that share a scale in a block-scaled cache: the largest power of two that divides the page size, at most 16."""
+    return _lib.lib().pd_scale_block_tokens(page_size)
+
+
+def append_target(k_cache, v_cache, block_table, start_pos, token_begin=None, slot_ids=None, k_scale=1.0, v_scale=1.0,
+                  d_k_scales=None, d_v_scales=None, d_block_scales=None):
+    """Where append_qkv puts k and v, from tensors: pools [num_pages, num_kv_heads, page_size, 128] (fp16, e4m3 or uint8),
+    block_table [num_slots, max_pages], start_pos [batch], token_begin [batch + 1] (None: one token each), slot_ids [batch]
+    (None: identity), all int32; scales float32, one kind of them (pd_append_target in the C header has the details).
+    Keeps the tensors alive."""
+    import torch
+    t = AppendTarget()
+    for name, pool in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if pool.dim() != 4 or pool.shape[3] != 128 or not pool.is_contiguous() or pool.shape != k_cache.shape or \
+                pool.dtype not in (torch.float16, torch.float8_e4m3fn, torch.uint8) or pool.dtype != k_cache.dtype:
+            raise InvalidArgument(f"{name} must be a dense [num_pages, num_kv_heads, page_size, 128] pool")
+    t.k_cache, t.v_cache = k_cache.data_ptr(), v_cache.data_ptr()
+    t.num_pages, heads, t.page_size = k_cache.shape[0], k_cache.shape[1], k_cache.shape[2]
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or not block_table.is_contiguous():
+        raise InvalidArgument("block_table must be a dense int32 matrix")
+    t.block_table, t.num_slots, t.block_table_stride = block_table.data_ptr(), block_table.shape[0], block_table.shape[1]
+    t.batch = start_pos.shape[0]
+    t.start_pos = _vector("start_pos", start_pos, torch.int32, t.batch)
+    t.token_begin = _vector("token_begin", token_begin, torch.int32, t.batch + 1)
+    t.slot_ids = _vector("slot_ids", slot_ids, torch.int32, t.batch)
+    if slot_ids is None and t.batch > t.num_slots:
+        raise InvalidArgument("more sequences than rows of the block table")
+    t.k_scale, t.v_scale = k_scale, v_scale
+    t.d_k_scales = _vector("d_k_scales", d_k_scales, torch.float32, heads)
+    t.d_v_scales = _vector("d_v_scales", d_v_scales, torch.float32, heads)
+    if d_block_scales is not None:
+        want = (t.num_pages, heads, t.page_size // scale_block_tokens(t.page_size), 2)
+        if d_block_scales.dtype != torch.float32 or tuple(d_block_scales.shape) != want or not d_block_scales.is_contiguous():
+            raise InvalidArgument(f"d_block_scales must be a dense float32 tensor of shape {want}")
+        t.d_block_scales = d_block_scales.data_ptr()
+    t._keep = (k_cache, v_cache, block_table, start_pos, token_begin, slot_ids, d_k_scales, d_v_scales, d_block_scales)
+    t._device = _device_index(t._keep)
+    return t
+
+
+def append_qkv(dtype, x, rope, target, d_q_out, stream=0):
+    """Norm, rotation and append in one pass (not in the reference): the q rows leave as dense fp16
+    [tokens, num_q_heads, 128], k and v go to their pages."""
+    device = getattr(target, "_device", None)
+    if device is not None and getattr(x, "_device", device) != device:
+        raise InvalidArgument("the rows and the cache are on different devices")
+    _check_device(device)
+    if hasattr(target, "_keep"):
+        pool = target._keep[0]
+        if pool.shape[1] != x.num_kv_heads or pool.element_size() != kv_dtype_bytes(dtype):
+            raise InvalidArgument("append_qkv: the pool's heads or type do not match")
+    if hasattr(d_q_out, "dim"):
+        _dense_fp16("d_q_out", d_q_out, x)
+    check(_lib.lib().pd_append_qkv(int(dtype), C.byref(x), rope._h if rope is not None else None, C.byref(target), _ptr(d_q_out),
+                                   stream))
+
+
+def _dense_fp16(name, q_out, x):
+    if q_out.element_size() != 2 or not q_out.is_contiguous() or q_out.numel() != x.num_tokens * x.num_q_heads * 128 or \
+            "bfloat" in str(q_out.dtype):
+        raise InvalidArgument(f"{name} must be dense fp16 [tokens, num_q_heads, 128]")
 
 
 class PagedKVCache:
@@ -368,6 +550,25 @@ class PagedKVCache:
         check(rc)
         return True
 
+    def append_qkv(self, slots, ns, x, rope, d_q_out, stream=0):
+        """append_qkv for slots of this cache (not in the reference), stream-ordered as append_batch: the rows of x are the
+        ns[0] tokens of slots[0], then the ns[1] of slots[1], ...; the rotated query rows go to d_q_out (fp16).
+        True when appended, False (nothing changed) when the pool cannot hold all of them."""
+        _check_device(getattr(x, "_device", None))
+        if hasattr(d_q_out, "dim"):
+            _dense_fp16("d_q_out", d_q_out, x)
+        s = np.ascontiguousarray(slots, dtype=np.int32)
+        n = np.ascontiguousarray(ns, dtype=np.int32)
+        if s.shape != n.shape or s.ndim != 1:
+            raise InvalidArgument("append_qkv: one token count per slot")
+        rc = _lib.lib().pd_cache_append_qkv(self._h, len(s), s.ctypes.data_as(C.POINTER(C.c_int)),
+                                            n.ctypes.data_as(C.POINTER(C.c_int)), C.byref(x),
+                                            rope._h if rope is not None else None, _ptr(d_q_out), stream)
+        if rc == _lib.PD_OUT_OF_PAGES:
+            return False
+        check(rc)
+        return True
+
     def release(self, slot):
         check(_lib.lib().pd_cache_release(self._h, slot))
 
@@ -384,6 +585,15 @@ class PagedKVCache:
                 raise _lib.InvalidArgument("set_head_scales: one scale per kv head is needed")
             arrays.append(a)
         check(_lib.lib().pd_cache_set_head_scales(self._h, *[None if a is None else a.ctypes.data for a in arrays]))
+
+    def set_block_scales(self, on=True):
+        """One fp8 scale per block of tokens (scale_block_tokens) and kv head, for K and for V, found while appending (not
+        in the reference); False restores the per-tensor scales.  Only while the cache is empty."""
+        check(_lib.lib().pd_cache_set_block_scales(self._h, int(bool(on))))
+
+    def block_scales(self):
+        """Device pointer of the scales [num_pages, num_kv_heads, page_size / block, 2], or None."""
+        return _lib.lib().pd_cache_block_scales(self._h)
 
     def plan(self, slots, num_q_heads, num_ctas=0, stream=0):
         s = np.ascontiguousarray(slots, dtype=np.int32)
@@ -446,7 +656,8 @@ class PagedKVCache:
         return out[:n].copy()
 
 
-__all__ = ["KVDtype", "DecodeParams", "DecodePlan", "DevicePlan", "PagedKVCache", "InvalidArgument", "LengthError",
+__all__ = ["ActDtype", "AppendTarget", "QKVParams", "Rope", "append_qkv", "append_target", "qk_norm_rope", "qkv_params",
+           "scale_block_tokens", "KVDtype", "DecodeParams", "DecodePlan", "DevicePlan", "PagedKVCache", "InvalidArgument", "LengthError",
            "kv_dtype_bytes", "kv_dtype_name", "tile_tokens", "wave_ctas", "default_ctas", "make_plan",
            "make_plan_tiled", "make_plan_weighted", "plan_from_arrays", "paged_decode", "paged_decode_static", "append_tokens", "stream_read", "kernel_status", "describe_launch", "set_head_fused", "head_fused",
            "set_adaptive_cut", "adaptive_cut", "adaptive_cut_reset", "adaptive_cut_refresh", "adaptive_cut_tables"]
