@@ -59,12 +59,13 @@ int fill_rows(const char* who, const pd_qkv* x, const pd_rope* rope, bool own_po
     return PD_OK;
 }
 
-// A row's heads go to as many warps as it takes to have about 16 per SM, at least one group of four heads each.
+// A row's units (four heads of q, k or v) go to as many warps as it takes to have about 16 per SM, at least one unit each.
 // (One token: 12 warps instead of one; 8192 tokens: one warp per row, which computes the row's sines once.)
-void spread_rows(pdk::RowArgs* a, int heads) {
-    const int groups = std::max(1, (heads + 3) / 4);
+void spread_rows(pdk::RowArgs* a, int kv_kinds) {
+    const int groups = std::max(1, (a->hq + 3) / 4 + kv_kinds * ((a->hkv + 3) / 4));
     const int wanted = 148 * 16;
     a->warps_per_row = std::max(1, std::min(groups, (wanted + a->tokens - 1) / std::max(1, a->tokens)));
+    if (const char* e = std::getenv("TUNE_UPW")) a->warps_per_row = std::max(a->warps_per_row, (groups + std::atoi(e) - 1) / std::atoi(e));
 }
 long long row_ctas(const pdk::RowArgs& a) {
     return (static_cast<long long>(a.tokens) * a.warps_per_row + pdk::ROWS_WARPS - 1) / pdk::ROWS_WARPS;
@@ -72,8 +73,15 @@ long long row_ctas(const pdk::RowArgs& a) {
 
 template<int SINK>
 void launch_rows(int act, const pdk::RowArgs& a, const pdk::RopeArgs& r, const pdk::PageArgs& t, long long ctas, cudaStream_t stream) {
-    if (act == PD_ACT_FP16) pdk::rows_kernel<__half, SINK><<<static_cast<unsigned>(ctas), pdk::ROWS_THREADS, 0, stream>>>(a, r, t);
-    else                    pdk::rows_kernel<__nv_bfloat16, SINK><<<static_cast<unsigned>(ctas), pdk::ROWS_THREADS, 0, stream>>>(a, r, t);
+    const unsigned grid = static_cast<unsigned>(ctas);
+    const bool halves = r.rotary_dim == 128 && !r.interleaved;
+    if (act == PD_ACT_FP16) {
+        if (halves) pdk::rows_kernel<__half, SINK, true><<<grid, pdk::ROWS_THREADS, 0, stream>>>(a, r, t);
+        else        pdk::rows_kernel<__half, SINK, false><<<grid, pdk::ROWS_THREADS, 0, stream>>>(a, r, t);
+    } else {
+        if (halves) pdk::rows_kernel<__nv_bfloat16, SINK, true><<<grid, pdk::ROWS_THREADS, 0, stream>>>(a, r, t);
+        else        pdk::rows_kernel<__nv_bfloat16, SINK, false><<<grid, pdk::ROWS_THREADS, 0, stream>>>(a, r, t);
+    }
 }
 
 // Appends rows to the pages; `a` and `t` are complete but for the work distribution.
@@ -85,17 +93,18 @@ int launch_append(int dtype, int act, pdk::RowArgs a, const pdk::RopeArgs& r, pd
         // blocks then start in different windows), a block's worth where they bring many.
         t.window = (t.token_begin || t.one_sequence) && a.tokens >= 8ll * t.batch ? pdk::MAX_BLOCK : 1;
         const long long windows = (a.tokens + static_cast<long long>(t.window) - 1) / t.window;
-        // 2 * hkv (head, K or V) units per block over 4 warps; short calls share them between CTAs
-        t.splits = static_cast<int>(std::max<long long>(1, std::min<long long>((2ll * a.hkv + pdk::ROWS_WARPS - 1) / pdk::ROWS_WARPS,
-                                                                               (148 * 4 + windows - 1) / windows)));
+        // 2 * hkv (head, K or V) units per block over the CTA's pairs of warps, or single warps where blocks get few rows;
+        // short calls share them between CTAs
+        const int teams = t.window == 1 ? pdk::ROWS_WARPS : pdk::ROWS_WARPS / 2;
+        t.splits = static_cast<int>(std::max<long long>(1, std::min<long long>((2ll * a.hkv + teams - 1) / teams, (148 * 5 + windows - 1) / windows)));
         const long long kv = windows * t.splits;
-        spread_rows(&a, a.hq);
+        spread_rows(&a, 0);
         const long long ctas = kv + (a.hq ? row_ctas(a) : 0);
         if (ctas > 0x7fffffff) return set_error(PD_LENGTH_ERROR, "append: too many tokens in one call");
         t.kv_ctas = static_cast<int>(kv);
         launch_rows<pdk::SINK_BLOCKS>(act, a, r, t, ctas, stream);
     } else {
-        spread_rows(&a, a.hq + 2 * a.hkv);
+        spread_rows(&a, 2);
         if (dtype == PD_FP16) launch_rows<pdk::SINK_FP16>(act, a, r, t, row_ctas(a), stream);
         else                  launch_rows<pdk::SINK_E4M3>(act, a, r, t, row_ctas(a), stream);
     }
@@ -155,7 +164,7 @@ int pd_qk_norm_rope(const pd_qkv* x, const pd_rope* rope, void* q_out, long long
         return set_error(PD_INVALID_ARGUMENT, "qk_norm_rope: in place needs the same row stride");
     a.q_out = q_out; a.q_out_stride = q_out_stride;
     a.k_out = k_out; a.k_out_stride = k_out_stride;
-    spread_rows(&a, a.hq + a.hkv);
+    spread_rows(&a, 1);
     launch_rows<pdk::SINK_DENSE>(x->act_dtype, a, r, pdk::PageArgs{}, row_ctas(a), static_cast<cudaStream_t>(stream));
     PD_CUDA(cudaGetLastError());
     return PD_OK;
