@@ -16,8 +16,16 @@ from ._lib import (InvalidArgument, LengthError, check, pd_append_target, pd_cac
                    pd_qkv)
 
 DecodeParams = pd_params
-QKVParams = pd_qkv
-AppendTarget = pd_append_target
+
+
+class QKVParams(pd_qkv):
+    """pd_qkv; qkv_params() fills one from tensors and notes what later calls check."""
+    _keep, _device, _dtype = (), None, None
+
+
+class AppendTarget(pd_append_target):
+    """pd_append_target; append_target() fills one from tensors and notes what later calls check."""
+    _keep, _device, _heads, _bytes = (), None, None, None
 
 
 class KVDtype(enum.IntEnum):
@@ -345,12 +353,19 @@ class Rope:
             self._h = None
 
 
+_current_device = None
+
+
 def _check_device(index):
     """The library works on the current device; tensors of another one are refused instead of faulting."""
-    if index is not None:
+    global _current_device
+    if index is None:
+        return
+    if _current_device is None:
         import torch
-        if torch.cuda.current_device() != index:
-            raise InvalidArgument(f"tensors on cuda:{index}, but the current device is cuda:{torch.cuda.current_device()}")
+        _current_device = torch.cuda.current_device
+    if _current_device() != index:
+        raise InvalidArgument(f"tensors on cuda:{index}, but the current device is cuda:{_current_device()}")
 
 
 def _device_index(tensors):
@@ -401,20 +416,31 @@ def qkv_params(q, k, v=None, q_norm=None, k_norm=None, eps=1e-6, positions=None)
     x.act_dtype = ActDtype.FP16 if k.dtype == torch.float16 else ActDtype.BF16
     x.num_tokens, x.num_kv_heads, x.head_dim, x.eps = tokens, k.shape[1], 128, eps
     x._keep = (q, k, v, q_norm, k_norm, positions)
-    x._device = _device_index(x._keep)
+    x._device, x._dtype = _device_index(x._keep), k.dtype
     return x
+
+
+def _out_rows(name, out, x, heads):
+    """(pointer, row stride) of an output of qk_norm_rope; 0: dense."""
+    if not hasattr(out, "stride"):
+        return _ptr(out), 0
+    steps, shape = out.stride(), out.shape
+    if steps[1:] == (128, 1) and shape == (x.num_tokens, heads, 128) and (out.dtype is x._dtype or x._dtype is None):
+        return out.data_ptr(), steps[0] if shape[0] > 1 else 0
+    if shape != (x.num_tokens, heads, 128) or (x._dtype is not None and out.dtype != x._dtype) or \
+            (out.numel() and (steps[2] != 1 or (heads > 1 and steps[1] != 128))):
+        raise InvalidArgument(f"{name} must be [tokens, heads, 128] like its input, with dense heads")
+    return out.data_ptr(), steps[0] if shape[0] > 1 else 0     # no element, or one head: the head's stride says nothing
 
 
 def qk_norm_rope(x, rope, d_q_out, d_k_out, stream=0):
     """Per-head RMS norm (where x has weights) and rotation (rope may be None) of the q and k rows in one pass (not in the
     reference).  Outputs like the inputs: tensors [tokens, heads, 128] (the inputs themselves: in place), or pointers
     to dense rows."""
-    _check_device(getattr(x, "_device", None))
-    strides = []
-    for name, out, heads in (("q_out", d_q_out, x.num_q_heads), ("k_out", d_k_out, x.num_kv_heads)):
-        strides.append(_rows_of(name, out, x._keep[1].dtype, x.num_tokens, heads) if hasattr(out, "dim") and hasattr(x, "_keep") else 0)
-    check(_lib.lib().pd_qk_norm_rope(C.byref(x), rope._h if rope is not None else None, _ptr(d_q_out), strides[0],
-                                     _ptr(d_k_out), strides[1], stream))
+    _check_device(x._device)
+    q, q_stride = _out_rows("q_out", d_q_out, x, x.num_q_heads)
+    k, k_stride = _out_rows("k_out", d_k_out, x, x.num_kv_heads)
+    check(_lib.lib().pd_qk_norm_rope(C.byref(x), rope._h if rope is not None else None, q, q_stride, k, k_stride, stream))
 
 
 def scale_block_tokens(page_size):
@@ -454,31 +480,40 @@ def append_target(k_cache, v_cache, block_table, start_pos, token_begin=None, sl
             raise InvalidArgument(f"d_block_scales must be a dense float32 tensor of shape {want}")
         t.d_block_scales = d_block_scales.data_ptr()
     t._keep = (k_cache, v_cache, block_table, start_pos, token_begin, slot_ids, d_k_scales, d_v_scales, d_block_scales)
-    t._device = _device_index(t._keep)
+    t._device, t._heads, t._bytes = _device_index(t._keep), heads, k_cache.element_size()
     return t
 
 
 def append_qkv(dtype, x, rope, target, d_q_out, stream=0):
     """Norm, rotation and append in one pass (not in the reference): the q rows leave as dense fp16
     [tokens, num_q_heads, 128], k and v go to their pages."""
-    device = getattr(target, "_device", None)
-    if device is not None and getattr(x, "_device", device) != device:
+    if x._device != target._device and x._device is not None and target._device is not None:
         raise InvalidArgument("the rows and the cache are on different devices")
-    _check_device(device)
-    if hasattr(target, "_keep"):
-        pool = target._keep[0]
-        if pool.shape[1] != x.num_kv_heads or pool.element_size() != kv_dtype_bytes(dtype):
-            raise InvalidArgument("append_qkv: the pool's heads or type do not match")
-    if hasattr(d_q_out, "dim"):
-        _dense_fp16("d_q_out", d_q_out, x)
-    check(_lib.lib().pd_append_qkv(int(dtype), C.byref(x), rope._h if rope is not None else None, C.byref(target), _ptr(d_q_out),
+    _check_device(target._device)
+    if target._heads is not None and (target._heads != x.num_kv_heads or target._bytes != (2 if dtype == KVDtype.FP16 else 1)):
+        raise InvalidArgument("append_qkv: the pool's heads or type do not match")
+    check(_lib.lib().pd_append_qkv(dtype, C.byref(x), rope._h if rope is not None else None, C.byref(target), _q_rows(d_q_out, x),
                                    stream))
 
 
-def _dense_fp16(name, q_out, x):
-    if q_out.element_size() != 2 or not q_out.is_contiguous() or q_out.numel() != x.num_tokens * x.num_q_heads * 128 or \
-            "bfloat" in str(q_out.dtype):
-        raise InvalidArgument(f"{name} must be dense fp16 [tokens, num_q_heads, 128]")
+_half = None
+
+
+def _torch_half():
+    global _half
+    if _half is None:
+        import torch
+        _half = torch.float16
+    return _half
+
+
+def _q_rows(out, x):
+    """Pointer of the fp16 query rows an append writes."""
+    if not hasattr(out, "is_contiguous"):
+        return _ptr(out)
+    if out.numel() != x.num_tokens * x.num_q_heads * 128 or not out.is_contiguous() or out.dtype != _torch_half():
+        raise InvalidArgument("d_q_out must be dense fp16 [tokens, num_q_heads, 128]")
+    return out.data_ptr()
 
 
 class PagedKVCache:
@@ -554,16 +589,15 @@ class PagedKVCache:
         """append_qkv for slots of this cache (not in the reference), stream-ordered as append_batch: the rows of x are the
         ns[0] tokens of slots[0], then the ns[1] of slots[1], ...; the rotated query rows go to d_q_out (fp16).
         True when appended, False (nothing changed) when the pool cannot hold all of them."""
-        _check_device(getattr(x, "_device", None))
-        if hasattr(d_q_out, "dim"):
-            _dense_fp16("d_q_out", d_q_out, x)
+        _check_device(x._device)
+        q_out = _q_rows(d_q_out, x)
         s = np.ascontiguousarray(slots, dtype=np.int32)
         n = np.ascontiguousarray(ns, dtype=np.int32)
         if s.shape != n.shape or s.ndim != 1:
             raise InvalidArgument("append_qkv: one token count per slot")
         rc = _lib.lib().pd_cache_append_qkv(self._h, len(s), s.ctypes.data_as(C.POINTER(C.c_int)),
                                             n.ctypes.data_as(C.POINTER(C.c_int)), C.byref(x),
-                                            rope._h if rope is not None else None, _ptr(d_q_out), stream)
+                                            rope._h if rope is not None else None, q_out, stream)
         if rc == _lib.PD_OUT_OF_PAGES:
             return False
         check(rc)

@@ -112,4 +112,11 @@ inline void paged_decode(KVDtype dtype, const DecodeParams& p, cudaStream_t stre
     check(pd_paged_decode(static_cast<int>(dtype), as_pd(p), stream));
 }
 
+// Not in the reference: the decode over an e4m3 cache with one scale per (block of tokens, kv head) for K and for V,
+// device floats [num_pages][num_kv_heads][page_size / block][2]; k_scale and v_scale of the params are ignored.
+inline void paged_decode_block_scaled(KVDtype dtype, const DecodeParams& p, int num_pages, const float* d_block_scales,
+                                      cudaStream_t stream = 0) {
+    check(pd_paged_decode_block_scaled(static_cast<int>(dtype), as_pd(p), num_pages, d_block_scales, stream));
+}
+
 }  // namespace decode

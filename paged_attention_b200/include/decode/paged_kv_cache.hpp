@@ -4,6 +4,7 @@
 // behind pd_cache_*; this class only keeps the reference's member names and error behaviour.
 
 #include "decode.hpp"
+#include "qkv_rows.hpp"
 
 #include <cstddef>
 #include <vector>
@@ -45,6 +46,17 @@ public:
         check(rc);
         return true;
     }
+    // Not in the reference: norm, rotation and append in one pass for many slots, stream-ordered.  x holds the
+    // n[0] rows of slots[0], then the n[1] rows of slots[1], ...; the fp16 query rows go to d_q_out.
+    bool append_qkv(const std::vector<int>& slots, const std::vector<int>& n, const QKVRows& x, const Rope* rope, half* d_q_out,
+                    cudaStream_t stream = 0) {
+        if (slots.size() != n.size()) throw std::invalid_argument("append_qkv: sizes differ");
+        const int rc = pd_cache_append_qkv(h_, static_cast<int>(slots.size()), slots.data(), n.data(), &x,
+                                           rope ? rope->handle() : nullptr, d_q_out, stream);
+        if (rc == PD_OUT_OF_PAGES) return false;
+        check(rc);
+        return true;
+    }
     void release(int slot) { check(pd_cache_release(h_, slot)); }
     // Not in the reference: one fp8 scale per kv head (num_kv_heads positive floats each) instead of the
     // per-tensor scales of the config; only while the cache holds no tokens.
@@ -53,6 +65,10 @@ public:
         check(pd_cache_set_head_scales(h_, k_scales.empty() ? nullptr : k_scales.data(),
                                        v_scales.empty() ? nullptr : v_scales.data()));
     }
+    // Not in the reference: one fp8 scale per (block of tokens, kv head) for K and for V, found while appending; only while
+    // the cache holds no tokens.
+    void set_block_scales(bool on = true) { check(pd_cache_set_block_scales(h_, on)); }
+    const float* block_scales() const { return pd_cache_block_scales(h_); }
     void shuffle_free_pages(unsigned seed) { pd_cache_shuffle_free_pages(h_, seed); }
 
     void plan(const std::vector<int>& slots, int num_q_heads, int num_ctas = 0, cudaStream_t stream = 0) {

@@ -6,6 +6,9 @@ Same constructor, `plan` / `run` split, argument order and checks; raw tensors, 
     dec.plan(seq_lens_cpu_int32, num_ctas=0)
     out = dec.run(q, k_cache, v_cache, block_table, seq_lens_dev, k_scale, v_scale)
 
+`run` also takes block_scales (not in the reference): float32 [pages, hkv, page_size / scale_block_tokens(page_size), 2], the
+scales of a block-scaled e4m3 cache, in place of k_scale / v_scale.
+
 q: [batch, hq, dim] fp16; k/v cache: [pages, hkv, page_size, dim] fp16 or float8_e4m3fn (or uint8 bytes);
 block_table: [batch, max_pages] int32; seq_lens_dev: [batch] int32 on the device.
 """
@@ -32,12 +35,17 @@ class Decoder:
         self._device_plan.upload(self._plan, self.hq // self.hkv, self.dim, torch.cuda.current_stream().cuda_stream)
         self._batch = len(lens)
 
-    def run(self, q, k_cache, v_cache, block_table, seq_lens_dev, k_scale=1.0, v_scale=1.0):
+    def run(self, q, k_cache, v_cache, block_table, seq_lens_dev, k_scale=1.0, v_scale=1.0, block_scales=None):
         import torch
         if not (q.is_cuda and q.dtype == torch.float16 and q.is_contiguous()):
             raise TypeError("run: q must be a contiguous CUDA fp16 tensor")
         if not (k_cache.is_contiguous() and v_cache.is_contiguous() and block_table.is_contiguous()):
             raise TypeError("run: caches and block table must be contiguous")
+        if block_scales is not None:
+            blocks = self.page // _d.scale_block_tokens(self.page)
+            if block_scales.dtype != torch.float32 or not (block_scales.is_cuda and block_scales.is_contiguous()) or \
+                    tuple(block_scales.shape) != (k_cache.size(0), self.hkv, blocks, 2):
+                raise TypeError("run: block_scales must be a contiguous CUDA float32 tensor [pages, hkv, blocks, 2]")
         if self._plan is None or q.size(0) != self._batch:
             raise ValueError("q batch does not match the plan")
         out = torch.empty_like(q)
@@ -50,7 +58,7 @@ class Decoder:
         p.sm_scale = 1.0 / math.sqrt(float(self.dim))
         p.k_scale, p.v_scale = float(k_scale), float(v_scale)
         self._device_plan.bind(p)
-        _d.paged_decode(self.dtype, p, torch.cuda.current_stream().cuda_stream, k_cache.size(0))
+        _d.paged_decode(self.dtype, p, torch.cuda.current_stream().cuda_stream, k_cache.size(0), d_block_scales=block_scales)
         return out
 
     @property

@@ -376,3 +376,74 @@ def test_cache_scale_modes_exclude_each_other(torch_cuda, pa):
     c.release(slot)
     c.set_block_scales(False)
     assert c.block_scales() is None
+
+
+def test_decoder_binding(torch_cuda, pa):
+    """The tensor binding takes the scales too, and checks them."""
+    from paged_attention_b200.torch_decode import Decoder
+    torch = torch_cuda
+    rng = np.random.default_rng(9)
+    lens = [70, 1, 333]
+    table, pages, bytes_, scales = random_cache(rng, lens, 4, 32, 2)
+    q = rng.standard_normal((3, 16, 128)).astype(np.float16)
+    want, tol = want_decode(q, bytes_, scales, table, lens, 32)
+    kc, vc = (torch.from_numpy(b).cuda() for b in bytes_)
+    d_scales, d_lens = torch.from_numpy(scales).cuda(), torch.tensor(lens, dtype=torch.int32, device="cuda")
+    dec = Decoder(16, 4, 128, 32, True)
+    dec.plan(torch.tensor(lens, dtype=torch.int32))
+    args = (torch.from_numpy(q).cuda(), kc, vc, torch.from_numpy(table).cuda(), d_lens)
+    out = dec.run(*args, block_scales=d_scales)
+    assert (np.abs(out.double().cpu().numpy() - want) <= tol).all()
+    for bad in (d_scales[:1], d_scales.half(), d_scales.transpose(1, 2), d_scales.cpu()):
+        with pytest.raises(TypeError):
+            dec.run(*args, block_scales=bad)
+
+
+def test_decode_replayed_in_a_graph_on_another_stream(torch_cuda, pa):
+    """Append and decode captured together and replayed as the sequences grow: lengths, positions and the plan are read on
+    the device."""
+    torch = torch_cuda
+    hq, hkv, ps, batch, steps = 8, 8, 16, 5, 40
+    pages = batch * 4
+    kc, vc, scales = pools(torch, pages, hkv, ps)
+    table = torch.randperm(pages, device="cuda").to(torch.int32).view(batch, 4).contiguous()
+    start = torch.tensor([0, 3, 15, 16, 9], dtype=torch.int32, device="cuda")
+    # the tokens before: one ragged append
+    first = Rows(torch, pa, int(start.sum()), hq, hkv, seed=1)
+    begin = torch.zeros(batch + 1, dtype=torch.int32, device="cuda")
+    begin[1:] = torch.cumsum(start, 0)
+    pa.append_qkv(FP8, first.params(), first.rope, pa.append_target(kc, vc, table, torch.zeros_like(start), begin, d_block_scales=scales),
+                  torch.empty(first.tokens, hq, 128, dtype=torch.float16, device="cuda"))
+    w = Rows(torch, pa, batch, hq, hkv, seed=2)
+    x, q = w.params(), torch.empty(batch, hq, 128, dtype=torch.float16, device="cuda")
+    out, lens = torch.empty_like(q), torch.empty_like(start)
+    target = pa.append_target(kc, vc, table, start, d_block_scales=scales)
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+
+    def step(p, dp):
+        pa.append_qkv(FP8, x, w.rope, target, q, s.cuda_stream)
+        torch.add(start, 1, out=lens)
+        dp.build(FP8, lens, batch, hq, hkv, 128, 0, None, s.cuda_stream)
+        dp.bind(p)
+        pa.paged_decode(FP8, p, s.cuda_stream, pages, d_block_scales=scales)
+        start.copy_(lens)
+
+    with torch.cuda.stream(s):
+        p, dp = bind(torch, pa, q, out, kc, vc, table, lens, [1] * batch, hq, hkv, ps)
+        step(p, dp)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            step(p, dp)
+    for i in range(steps):
+        w.k.mul_(1.07)          # in place: the captured rows grow, and scales with them
+        w.v.mul_(1.07)
+        g.replay()
+        if i % 13 == 0 or i == steps - 1:
+            torch.cuda.synchronize()
+            assert pa.kernel_status() == 0
+            want, tol = want_decode(q.cpu().numpy(), (kc.cpu().numpy(), vc.cpu().numpy()), scales.cpu().numpy(), table.cpu().numpy(),
+                                    lens.tolist(), ps)
+            assert (np.abs(out.double().cpu().numpy() - want) <= tol).all()
+    assert lens.tolist() == [n + 1 + steps for n in [0, 3, 15, 16, 9]]
