@@ -412,7 +412,9 @@ typedef struct pd_append_target {
 } pd_append_target;
 
 /* Norm, rotation and append in one pass: q leaves as dense fp16 rows [num_tokens][num_q_heads][head_dim] (what the
- * decode reads), k and v go to their pages.  Does not wait. */
+ * decode reads), k and v go to their pages.  bf16 values beyond fp16's range become infinities in q_out and in an fp16
+ * cache.  q_out must not overlap the rows of x.  Does not wait.  As with pd_paged_decode, the first call on a device sets
+ * up the status word and belongs before any stream capture. */
 int pd_append_qkv(int dtype, const pd_qkv* x, const pd_rope* rope, const pd_append_target* t, void* q_out, void* stream);
 
 /* decode::PagedKVCache (src/decode/paged_kv_cache.hpp:31-73). */
@@ -443,6 +445,8 @@ int    pd_cache_release(pd_cache* c, int slot);
 int    pd_cache_set_head_scales(pd_cache* c, const float* k_scales, const float* v_scales);
 /* One scale per (block of tokens, kv head) for K and for V instead of the config's per-tensor scales (fp8 cache; on = 0:
  * back to those).  Every later append quantises with them, as pd_append_qkv does, and every later run reads them.
+ * The params of such a cache (pd_cache_params) carry NaN as k_scale and v_scale, which this decode ignores and any
+ * decode that does not take the block scales turns into NaN instead of silently wrong numbers.
  * Only while the cache holds no tokens and without head scales.  Adds 8 bytes per block and kv head, which
  * pd_cache_bytes_per_page and pd_cache_total_bytes do not count.  No counterpart in the reference. */
 int    pd_cache_set_block_scales(pd_cache* c, int on);

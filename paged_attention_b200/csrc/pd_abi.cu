@@ -1889,6 +1889,7 @@ int pd_cache_params(const pd_cache* c, pd_params* p) {
     p->sm_scale           = 1.0f / std::sqrt(static_cast<float>(c->cfg.head_dim));
     p->k_scale            = fp8 ? c->cfg.k_scale : 1.0f;
     p->v_scale            = fp8 ? c->cfg.v_scale : 1.0f;
+    if (c->d_block_scales) p->k_scale = p->v_scale = std::nanf("");   // only the block-scaled decode, which ignores them, may run
     return PD_OK;
 }
 

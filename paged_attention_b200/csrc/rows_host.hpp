@@ -8,8 +8,6 @@ struct pd_rope {
 
 namespace {
 
-constexpr double TWO_PI = 6.283185307179586476925286766559;
-
 // Largest power of two that divides the page, at most 16: blocks tile every page, whatever its size.
 int scale_block_log2(int page_size) {
     int lb = 0;
@@ -17,6 +15,7 @@ int scale_block_log2(int page_size) {
     return lb;
 }
 
+bool unaligned4(const void* p) { return reinterpret_cast<uintptr_t>(p) % 4 != 0; }
 bool unaligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; }
 
 // One of q, k, v: rows of heads * 128 elements, `stride` elements apart (0: dense).
@@ -47,6 +46,7 @@ int fill_rows(const char* who, const pd_qkv* x, const pd_rope* rope, bool own_po
     if ((x->q_norm || x->k_norm) && !(x->eps >= 0.f && std::isfinite(x->eps)))
         return set_error(PD_INVALID_ARGUMENT, "%s: eps must be finite and not negative", who);
     *r = rope ? rope->args : pdk::RopeArgs{};
+    if (unaligned4(x->positions)) return set_error(PD_INVALID_ARGUMENT, "%s: positions must be 4-byte aligned", who);
     if (rope && rope->args.rotary_dim) {
         if (!x->positions && !own_positions) return set_error(PD_INVALID_ARGUMENT, "%s: a rotation needs positions", who);
         if (x->positions && x->num_axes < rope->args.axes)
@@ -59,13 +59,13 @@ int fill_rows(const char* who, const pd_qkv* x, const pd_rope* rope, bool own_po
     return PD_OK;
 }
 
-// A row's units (four heads of q, k or v) go to as many warps as it takes to have about 16 per SM, at least one unit each.
-// (One token: 12 warps instead of one; 8192 tokens: one warp per row, which computes the row's sines once.)
+// A row's units (four heads of q, k or v) go to as many warps as still fit on the SMs at once, 16 of the 20 an SM takes: one
+// token goes to 12 warps instead of one, 1000 to two warps each, and from 2400 on each row to one warp, which then computes
+// the row's sines once.  (A second wave costs more than longer rows: 2000 rows of 40 heads took 12.8 us with two warps each, 10.0
+// with one; 600 rows 5.7 us with one each, 4.8 with four.)
 void spread_rows(pdk::RowArgs* a, int kv_kinds) {
-    const int groups = std::max(1, (a->hq + 3) / 4 + kv_kinds * ((a->hkv + 3) / 4));
-    const int wanted = 148 * 16;
-    a->warps_per_row = std::max(1, std::min(groups, (wanted + a->tokens - 1) / std::max(1, a->tokens)));
-    if (const char* e = std::getenv("TUNE_UPW")) a->warps_per_row = std::max(a->warps_per_row, (groups + std::atoi(e) - 1) / std::atoi(e));
+    const int units = std::max(1, (a->hq + 3) / 4 + kv_kinds * ((a->hkv + 3) / 4));
+    a->warps_per_row = std::max(1, std::min(units, 148 * 16 / std::max(1, a->tokens)));
 }
 long long row_ctas(const pdk::RowArgs& a) {
     return (static_cast<long long>(a.tokens) * a.warps_per_row + pdk::ROWS_WARPS - 1) / pdk::ROWS_WARPS;
@@ -93,10 +93,12 @@ int launch_append(int dtype, int act, pdk::RowArgs a, const pdk::RopeArgs& r, pd
         // blocks then start in different windows), a block's worth where they bring many.
         t.window = (t.token_begin || t.one_sequence) && a.tokens >= 8ll * t.batch ? pdk::MAX_BLOCK : 1;
         const long long windows = (a.tokens + static_cast<long long>(t.window) - 1) / t.window;
-        // 2 * hkv (head, K or V) units per block over the CTA's pairs of warps, or single warps where blocks get few rows;
-        // short calls share them between CTAs
+        // The 2 * hkv (head, K or V) units of a block go to the CTA's pairs of warps, or single warps where blocks get few rows.
+        // Calls with few windows share a window between CTAs until there are about two per SM: with more than fit on the
+        // SMs beside the q rows a second wave starts (128 sequences of one token: 5.6 us with one CTA per window, 4.6 with two,
+        // 5.6 with four; 1000 tokens of one sequence: 15.0 us with one, 9.5 with four).
         const int teams = t.window == 1 ? pdk::ROWS_WARPS : pdk::ROWS_WARPS / 2;
-        t.splits = static_cast<int>(std::max<long long>(1, std::min<long long>((2ll * a.hkv + teams - 1) / teams, (148 * 5 + windows - 1) / windows)));
+        t.splits = static_cast<int>(std::max<long long>(1, std::min<long long>((2ll * a.hkv + teams - 1) / teams, 148 * 2 / windows)));
         const long long kv = windows * t.splits;
         spread_rows(&a, 0);
         const long long ctas = kv + (a.hq ? row_ctas(a) : 0);
@@ -188,6 +190,9 @@ int pd_append_qkv(int dtype, const pd_qkv* x, const pd_rope* rope, const pd_appe
     if (int rc = check_rows(who, "q_out", q_out, &out_stride, a.hq)) return rc;
     if (!t->k_cache || !t->v_cache || !t->block_table || !t->start_pos) return set_error(PD_INVALID_ARGUMENT, "append_qkv: null device pointer");
     if (unaligned16(t->k_cache) || unaligned16(t->v_cache)) return set_error(PD_INVALID_ARGUMENT, "append_qkv: pools must be 16-byte aligned");
+    if (unaligned4(t->block_table) || unaligned4(t->start_pos) || unaligned4(t->token_begin) || unaligned4(t->slot_ids) ||
+        unaligned4(t->d_k_scales) || unaligned4(t->d_v_scales))
+        return set_error(PD_INVALID_ARGUMENT, "append_qkv: lists and scales must be 4-byte aligned");
     if (t->d_block_scales) {
         if (dtype != PD_FP8_E4M3) return set_error(PD_INVALID_ARGUMENT, "append_qkv: only an fp8 cache is quantised");
         if (t->d_k_scales || t->d_v_scales) return set_error(PD_INVALID_ARGUMENT, "append_qkv: head scales and block scales exclude each other");

@@ -330,7 +330,7 @@ struct RowSmem {
 struct BlockSmem {
     uint4  map[MAX_BLOCK][8][8];                    // the block's rows: (diag, cross) of a lane's pair i at [row][i][lane of 8]
     uint4  slots[ROWS_WARPS][2][2][2][32];          // [warp][unit on its way][four rows][chunk][lane]
-    float  top[ROWS_WARPS / 2][2][2];               // [pair of warps][unit parity][warp]: largest magnitude of the warp's rows
+    float  top[ROWS_WARPS / 2][2][2];               // [pair of warps][parity][warp]: largest magnitude of the warp's rows
 };
 
 // k and v of one block of at most 16 tokens: all its new rows meet in two warps per (head, K or V), eight rows each, which
@@ -352,6 +352,7 @@ __device__ __forceinline__ void write_blocks(const RowArgs& a, const RopeArgs& r
     const bool mapped = rotary || a.k_norm != nullptr;
     const Chunks ch = HALVES ? Chunks{j, j + 8, true} : chunks_of(j, rope.rotary_dim);
     const int stop = min((window + 1) * t.window, a.tokens);
+    int parity = 0;                                                           // of sm.top, over all blocks of the window
     for (int row = window * t.window; row < stop;) {
         const Place p = locate(t, row, a.tokens, lane);
         if (p.slot < 0) { row = max(row + 1, p.end); continue; }              // no sequence's row, or a skipped sequence
@@ -463,9 +464,10 @@ __device__ __forceinline__ void write_blocks(const RowArgs& a, const RopeArgs& r
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                 if (paired) {                                                 // both warps of a pair take the same units
-                    if (lane == 0) sm.top[team][slot][half] = top;
+                    if (lane == 0) sm.top[team][parity][half] = top;
                     asm volatile("bar.sync %0, 64;" :: "r"(1 + team) : "memory");
-                    top = fmaxf(sm.top[team][slot][0], sm.top[team][slot][1]);
+                    top = fmaxf(sm.top[team][parity][0], sm.top[team][parity][1]);
+                    parity ^= 1;   // the other warp may still be reading; it has done so when the next barrier is passed
                 }
                 slot ^= 1;
                 // smallest power of two with top / scale <= 448 = 1.75 * 2^8

@@ -381,7 +381,11 @@ def _rows_of(name, x, dtype=None, tokens=None, heads=None):
         raise InvalidArgument(f"{name} must be [tokens, heads, 128] with dense heads")
     if (dtype is not None and x.dtype != dtype) or (tokens is not None and x.shape[0] != tokens) or (heads is not None and x.shape[1] != heads):
         raise InvalidArgument(f"{name} does not match the other rows")
-    return x.stride(0) if x.shape[0] > 1 else 0     # one row, or none: the stride says nothing
+    if x.shape[0] < 2 or x.shape[1] == 0:
+        return 0                                    # one row, or none: the stride says nothing
+    if x.stride(0) < x.shape[1] * 128:
+        raise InvalidArgument(f"{name}: rows overlap (a broadcast tensor?)")
+    return x.stride(0)
 
 
 def _vector(name, x, dtype, n):
@@ -410,7 +414,7 @@ def qkv_params(q, k, v=None, q_norm=None, k_norm=None, eps=1e-6, positions=None)
         if p.dtype != torch.int32 or p.dim() != 2 or p.shape[1] != tokens or (tokens > 1 and p.stride(1) != 1):
             raise InvalidArgument("positions must be int32 [tokens] or [axes, tokens], dense along the tokens")
         if p.shape[0] > 1 and p.stride(0) < tokens:
-            p = p.contiguous()      # a broadcast axis
+            raise InvalidArgument("positions of a broadcast axis: make them dense")
         x.positions, x.num_axes, x.positions_stride = p.data_ptr(), p.shape[0], p.stride(0) if p.shape[0] > 1 else tokens
         positions = p
     x.act_dtype = ActDtype.FP16 if k.dtype == torch.float16 else ActDtype.BF16
@@ -425,12 +429,18 @@ def _out_rows(name, out, x, heads):
     if not hasattr(out, "stride"):
         return _ptr(out), 0
     steps, shape = out.stride(), out.shape
-    if steps[1:] == (128, 1) and shape == (x.num_tokens, heads, 128) and (out.dtype is x._dtype or x._dtype is None):
-        return out.data_ptr(), steps[0] if shape[0] > 1 else 0
-    if shape != (x.num_tokens, heads, 128) or (x._dtype is not None and out.dtype != x._dtype) or \
-            (out.numel() and (steps[2] != 1 or (heads > 1 and steps[1] != 128))):
-        raise InvalidArgument(f"{name} must be [tokens, heads, 128] like its input, with dense heads")
-    return out.data_ptr(), steps[0] if shape[0] > 1 else 0     # no element, or one head: the head's stride says nothing
+    if shape != (x.num_tokens, heads, 128) or (x._dtype is not None and out.dtype != x._dtype):
+        raise InvalidArgument(f"{name} must be [tokens, heads, 128] like its input")
+    if x._device is not None and out.get_device() != x._device:
+        raise InvalidArgument(f"{name} is on another device than the rows")
+    if heads and shape[0]:
+        if steps[2] != 1 or (heads > 1 and steps[1] != 128):
+            raise InvalidArgument(f"{name}: heads must be dense")
+        if shape[0] > 1:
+            if steps[0] < heads * 128:
+                raise InvalidArgument(f"{name}: rows overlap (a broadcast tensor?)")
+            return out.data_ptr(), steps[0]
+    return out.data_ptr(), 0                        # one row, or none: the stride says nothing
 
 
 def qk_norm_rope(x, rope, d_q_out, d_k_out, stream=0):
@@ -513,6 +523,8 @@ def _q_rows(out, x):
         return _ptr(out)
     if out.numel() != x.num_tokens * x.num_q_heads * 128 or not out.is_contiguous() or out.dtype != _torch_half():
         raise InvalidArgument("d_q_out must be dense fp16 [tokens, num_q_heads, 128]")
+    if x._device is not None and out.get_device() != x._device:
+        raise InvalidArgument("d_q_out is on another device than the rows")
     return out.data_ptr()
 
 

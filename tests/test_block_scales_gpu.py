@@ -447,3 +447,40 @@ def test_decode_replayed_in_a_graph_on_another_stream(torch_cuda, pa):
                                     lens.tolist(), ps)
             assert (np.abs(out.double().cpu().numpy() - want) <= tol).all()
     assert lens.tolist() == [n + 1 + steps for n in [0, 3, 15, 16, 9]]
+
+
+@pytest.mark.parametrize("hkv", [1, 3, 5])
+def test_many_short_sequences_of_plain_rows(hkv, torch_cuda, pa):
+    """Blocks of nine and more rows, several to a window of rows, neither normed nor rotated: pairs of warps meet over every
+    (head, K or V) of one block after the other.  V scales are exact here, so every byte is determined."""
+    torch = torch_cuda
+    new = [9, 16, 12, 10, 9, 9, 15, 11] * 40
+    g = torch.Generator(device="cuda").manual_seed(hkv)
+    tokens = sum(new)
+    k, v = (torch.randn(tokens, hkv, 128, generator=g, device="cuda").mul_(torch.exp2(torch.randint(-6, 7, (tokens, hkv, 1), generator=g, device="cuda"))).half()
+            for _ in range(2))
+    kc, vc, scales = pools(torch, len(new), hkv, 16)
+    table = torch.randperm(len(new), generator=g, device="cuda").to(torch.int32)[:, None].contiguous()
+    begin = torch.tensor([0] + list(np.cumsum(new)), dtype=torch.int32, device="cuda")
+    t = pa.append_target(kc, vc, table, torch.zeros(len(new), dtype=torch.int32, device="cuda"), begin, d_block_scales=scales)
+    for _ in range(5):
+        pa.append_qkv(FP8, pa.qkv_params(None, k, v), None, t, None)
+    assert pa.kernel_status() == 0
+    page, at = table[:, 0].tolist(), 0
+    got_s = scales.cpu().numpy()
+    for which, (pool, x) in enumerate(((kc, k), (vc, v))):
+        raw, x64, at = pool.cpu().numpy(), x.double().cpu().numpy(), 0
+        for p, n in zip(page, new):
+            for h in range(hkv):
+                s = ro.need_scale(np.abs(x64[at:at + n, h]).max())
+                assert got_s[p, h, 0, which] == s
+                assert np.array_equal(raw[p, h, :n], encode(x64[at:at + n, h] / s))
+            at += n
+
+
+def test_params_of_a_block_scaled_cache_do_not_fit_another_decode(torch_cuda, pa):
+    torch = torch_cuda
+    c = pa.PagedKVCache(pa.PagedKVCache.Config(4, 16, 8, 128, 2, 2, pa.KVDtype.FP8_E4M3))
+    assert c.params().k_scale == 1.0
+    c.set_block_scales()
+    assert np.isnan(c.params().k_scale) and np.isnan(c.params().v_scale)

@@ -46,7 +46,7 @@ def test_rope_accepts(pa):
     (dict(act_dtype=2), "dtype"), (dict(head_dim=64), "head_dim"), (dict(num_tokens=-1), "count"), (dict(num_q_heads=-1), "count"),
     (dict(q=None), "q is null"), (dict(k=None), "k is null"), (dict(q=(1 << 20) + 8), "aligned"), (dict(q_stride=8 * 128 + 4), "multiples"),
     (dict(q_stride=7 * 128), "at least"), (dict(k_stride=-256), "at least"), (dict(q_norm=8), "aligned"),
-    (dict(q_norm=16, eps=-1.0), "eps"), (dict(k_norm=16, eps=float("nan")), "eps"), (dict(positions=None), "positions"),
+    (dict(q_norm=16, eps=-1.0), "eps"), (dict(k_norm=16, eps=float("nan")), "eps"), (dict(positions=None), "positions"), (dict(positions=(1 << 16) + 2), "aligned"),
     (dict(num_axes=1, axes3=True), "axes"), (dict(num_axes=3, positions_stride=4, axes3=True), "positions_stride")])
 def test_qk_norm_rope_refusals(bad, match, pa):
     bad = dict(dict(positions=1 << 16, num_axes=1, positions_stride=5), **bad)
@@ -68,6 +68,7 @@ def test_qk_norm_rope_output_refusals(pa):
     (dict(page_size=0), "positive"), (dict(num_pages=0), "positive"), (dict(num_slots=0), "positive"), (dict(block_table_stride=0), "positive"),
     (dict(batch=-1), "positive"), (dict(k_cache=None), "null"), (dict(block_table=None), "null"), (dict(start_pos=None), "null"),
     (dict(v_cache=(5 << 20) + 8), "aligned"), (dict(k_scale=0.0), "scales"), (dict(v_scale=float("nan")), "scales"),
+    (dict(block_table=(6 << 20) + 1), "aligned"), (dict(token_begin=(6 << 20) + 2), "aligned"), (dict(d_v_scales=6), "aligned"),
     (dict(d_block_scales=1 << 16, d_k_scales=1 << 16), "exclude"), (dict(d_block_scales=(1 << 16) + 4), "aligned")])
 def test_append_qkv_refusals(bad, match, pa):
     with pytest.raises(pa.InvalidArgument, match=match):
@@ -110,6 +111,8 @@ def test_builders_check_their_tensors(pa):
                dict(q=None, k=h(3, 2, 128, dtype=torch.float32)), dict(q=None, k=h(3, 2, 256)[:, :, ::2]), dict(q=None, k=h(3, 4, 128)[:, ::2]),
                dict(q=None, k=h(3, 2, 128), v=h(3, 1, 128)), dict(q=None, k=h(3, 2, 128), k_norm=h(128, dtype=torch.float32)),
                dict(q=None, k=h(3, 2, 128), positions=torch.zeros(3)), dict(q=None, k=h(3, 2, 128), positions=torch.zeros(2, dtype=torch.int32)),
+               dict(q=None, k=h(1, 2, 128).expand(3, 2, 128)), dict(q=h(3, 4, 128), k=h(3, 1, 128).expand(3, 2, 128)),
+               dict(q=None, k=h(3, 2, 128), positions=torch.zeros(1, 3, dtype=torch.int32).expand(2, 3)),
                dict(q=None, k=h(3, 2, 128))):                                   # the last: not on a GPU
         with pytest.raises(pa.InvalidArgument):
             pa.qkv_params(**kw)
@@ -132,3 +135,18 @@ def test_oracle_e4m3_rounding():
     x = np.concatenate([np.linspace(0, 0.05, 2001), np.linspace(0, 447, 4001), (ro.e4m3_values()[1:] + ro.e4m3_values()[:-1]) / 2])
     x = x.astype(np.float32).astype(np.float64)
     assert np.array_equal(ro.round_e4m3(x), torch.from_numpy(x).to(torch.float32).to(torch.float8_e4m3fn).double().numpy())
+
+
+def test_outputs_are_checked(pa):
+    torch = pytest.importorskip("torch")
+    x = rows(pa, num_tokens=3, num_q_heads=2, positions=1 << 16, num_axes=1)
+    x._dtype = torch.float16
+    h = lambda *s, dtype=torch.float16: torch.zeros(*s, dtype=dtype)   # noqa: E731
+    k = 9 << 20
+    for q in (h(3, 2, 64), h(2, 2, 128), h(3, 2, 128, dtype=torch.bfloat16), h(1, 2, 128).expand(3, 2, 128), h(3, 1, 128).expand(3, 2, 128),
+              h(3, 4, 128)[:, ::2], h(3, 2, 256)[:, :, ::2]):
+        with pytest.raises(pa.InvalidArgument):
+            pa.qk_norm_rope(x, None, q, k)
+    for q in (h(3, 2, 64), h(4, 2, 128), h(3, 2, 128, dtype=torch.bfloat16), h(3, 4, 128)[:, :2]):
+        with pytest.raises(pa.InvalidArgument):
+            pa.append_qkv(pa.KVDtype.FP16, x, None, target(pa), q)
