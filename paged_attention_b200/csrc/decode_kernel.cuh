@@ -81,7 +81,10 @@ struct HeadScales {
 // Scales of a block-scaled e4m3 cache: float pairs (K, V) at [page][kv head][block of the page]; a block is the largest
 // power of two of tokens that divides the page size, at most 16.  The producer warp brings a tile's pairs into the
 // tile's stage with 8-byte asynchronous copies that arrive on the same barrier as the tile: 8 bytes beside 4 KB of K and V per
-// 16 tokens and head.
+// 16 tokens and head.  Against the same decode with one scale per tensor, measured on B200: 128 x 4096 tokens 163.6 us and
+// 162.1, a ragged 256 x 4100 (64 query heads) 333.8 and 329.2 (both at the copy rate of the traffic); steps too short to be
+// bound by memory pay more for the work per tile: 16 x 4096 with groups of 8 32.4 us and 31.0, 32 x 1024 with 4 kv heads 12.9 and
+// 12.1.  Fetching the scales ahead of the products, or cheaper reciprocals, changed none of these by more than 1 %.
 struct BlockScales {
     const float2* scales;
     int log2_block;

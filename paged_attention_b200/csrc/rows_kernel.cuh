@@ -17,9 +17,10 @@
 // warp (two frequencies per lane) and shared by all heads the warp takes.
 //
 // Bound: memory, one read of the rows and one write of the results.  Measured on B200 against that traffic at the
-// measured copy rate (6.55 TB/s): 8192 bf16 rows of 40 heads with norm 29.5 us (87 %), 20001 rows of 72 heads 114 us
-// (99 %), prompts of 33,000 rows of 80 heads into an fp16 cache 206 us (99 %), ragged chunks into an e4m3 cache 48 us
-// (88 %), into a block-scaled one 66 us (81 %); one row 2.5 us, a launch.
+// measured copy rate (6.55 TB/s): 8192 bf16 rows of 40 heads with norm 29.5 us (87 %), 65536 of them 201 us (102 %), 20001
+// rows of 72 heads 114 us (99 %), prompts of 33,000 rows of 80 heads into an fp16 cache 206 us (99 %), ragged chunks of
+// 12,000 rows into an e4m3 cache 48 us (88 %), of 15,500 into a block-scaled one 66 us (81 %; 87 % at four times the rows); one
+// row 2.5 us, a launch.  What is missing at the smaller sizes is 4 us of launch, first loads and last stores.
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -365,6 +366,8 @@ __device__ __forceinline__ void write_blocks(const RowArgs& a, const RopeArgs& r
         const int page = spot.page, off = spot.off;
         if (page < 0) continue;
 
+        float* scales = t.block_scales + 2 * (static_cast<size_t>(page) * a.hkv * per_page + (off >> t.log2_block));   // of kv head 0
+        const size_t row0 = (static_cast<size_t>(page) * a.hkv * t.page_size + off) * 128;                         // first row, kv head 0
         const bool paired = n > 8;
         const int half = paired ? warp & 1 : 0, mine = 8 * half + (lane >> 3);   // this lane's rows of the block: mine, mine + 4
         const size_t from = t.k_src ? first_row - p.begin : first_row;
@@ -424,7 +427,7 @@ __device__ __forceinline__ void write_blocks(const RowArgs& a, const RopeArgs& r
 #pragma unroll 1
             for (; u < end; u += step) {
                 const int h = is_v ? u - a.hkv : u;
-                float* scale_at = t.block_scales + 2 * ((static_cast<size_t>(page) * a.hkv + h) * per_page + (off >> t.log2_block)) + is_v;
+                float* scale_at = scales + h * 2 * per_page + is_v;
                 float old = inside ? *scale_at : 0.f;
                 fetch(u + step, slot ^ 1);
                 cp_async_wait<1>();
@@ -461,8 +464,7 @@ __device__ __forceinline__ void write_blocks(const RowArgs& a, const RopeArgs& r
                         top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
                     }
                 }
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));   // not negative: ordered like its bits
                 if (paired) {                                                 // both warps of a pair take the same units
                     if (lane == 0) sm.top[team][parity][half] = top;
                     asm volatile("bar.sync %0, 64;" :: "r"(1 + team) : "memory");
@@ -477,18 +479,18 @@ __device__ __forceinline__ void write_blocks(const RowArgs& a, const RopeArgs& r
                 const float need = __uint_as_float(static_cast<unsigned>(e + 127) << 23);
                 old = old > 0.f ? old : 0.f;
                 const float scale = fmaxf(old, need), inv = __fdividef(1.f, scale);   // exact for powers of two
-                unsigned char* dst = static_cast<unsigned char*>(is_v ? t.v_cache : t.k_cache)
-                    + ((static_cast<size_t>(page) * a.hkv + h) * t.page_size + off) * 128;
+                unsigned char* head = static_cast<unsigned char*>(is_v ? t.v_cache : t.k_cache) + row0 + static_cast<size_t>(h) * t.page_size * 128;
+                unsigned char* dst = head + mine * 128 + ch.a * 8;
 #pragma unroll
                 for (int s = 0; s < 2; s++) {
                     if (4 * s + mine >= n) break;
                     scale_by(x[s], inv);
-                    *reinterpret_cast<uint2*>(dst + (4 * s + mine) * 128 + ch.a * 8) = quant8(x[s], 0);
-                    *reinterpret_cast<uint2*>(dst + (4 * s + mine) * 128 + ch.b * 8) = quant8(x[s], 4);
+                    *reinterpret_cast<uint2*>(dst + 512 * s)         = quant8(x[s], 0);
+                    *reinterpret_cast<uint2*>(dst + 512 * s + b_off) = quant8(x[s], 4);
                 }
                 if (inside && scale > old) {                                  // warp-uniform
                     const float ratio = old * inv;
-                    unsigned char* was = dst - inside * 128;
+                    unsigned char* was = head - inside * 128;
                     for (int r = mine; r < (paired ? min(block, 8 * half + 8) : block); r += 4) {
                         if (r >= inside && r < inside + n) continue;          // just written
                         uint4* at = reinterpret_cast<uint4*>(was + r * 128) + j;
