@@ -73,15 +73,18 @@ long long row_ctas(const pdk::RowArgs& a) {
 
 template<int SINK>
 void launch_rows(int act, const pdk::RowArgs& a, const pdk::RopeArgs& r, const pdk::PageArgs& t, long long ctas, cudaStream_t stream) {
-    const unsigned grid = static_cast<unsigned>(ctas);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+    cfg.blockDim = dim3(pdk::ROWS_THREADS);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
     const bool halves = r.rotary_dim == 128 && !r.interleaved;
-    if (act == PD_ACT_FP16) {
-        if (halves) pdk::rows_kernel<__half, SINK, true><<<grid, pdk::ROWS_THREADS, 0, stream>>>(a, r, t);
-        else        pdk::rows_kernel<__half, SINK, false><<<grid, pdk::ROWS_THREADS, 0, stream>>>(a, r, t);
-    } else {
-        if (halves) pdk::rows_kernel<__nv_bfloat16, SINK, true><<<grid, pdk::ROWS_THREADS, 0, stream>>>(a, r, t);
-        else        pdk::rows_kernel<__nv_bfloat16, SINK, false><<<grid, pdk::ROWS_THREADS, 0, stream>>>(a, r, t);
-    }
+    if (act == PD_ACT_FP16) cudaLaunchKernelEx(&cfg, halves ? pdk::rows_kernel<__half, SINK, true> : pdk::rows_kernel<__half, SINK, false>, a, r, t);
+    else cudaLaunchKernelEx(&cfg, halves ? pdk::rows_kernel<__nv_bfloat16, SINK, true> : pdk::rows_kernel<__nv_bfloat16, SINK, false>, a, r, t);
 }
 
 // Appends rows to the pages; `a` and `t` are complete but for the work distribution.

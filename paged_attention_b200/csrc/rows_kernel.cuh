@@ -17,10 +17,10 @@
 // warp (two frequencies per lane) and shared by all heads the warp takes.
 //
 // Bound: memory, one read of the rows and one write of the results.  Measured on B200 against that traffic at the
-// measured copy rate (6.55 TB/s): 8192 bf16 rows of 40 heads with norm 29.5 us (87 %), 65536 of them 201 us (102 %), 20001
-// rows of 72 heads 114 us (99 %), prompts of 33,000 rows of 80 heads into an fp16 cache 206 us (99 %), ragged chunks of
-// 12,000 rows into an e4m3 cache 48 us (88 %), of 15,500 into a block-scaled one 66 us (81 %; 87 % at four times the rows); one
-// row 2.5 us, a launch.  What is missing at the smaller sizes is 4 us of launch, first loads and last stores.
+// measured copy rate (6.55 TB/s): 8192 bf16 rows of 40 heads with norm 28.8 us (89 %), 65536 of them 201 us (102 %), 20001
+// rows of 72 heads 113 us (99 %), prompts of 33,000 rows of 80 heads into an fp16 cache 206 us (100 %), ragged chunks of
+// 12,000 rows into an e4m3 cache 47 us (88 %), of 15,500 into a block-scaled one 65 us (82 %; 87 % at four times the rows); one
+// row 2.3 us, a launch.  What is missing at the smaller sizes is 3 us of first loads and last stores.
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -530,6 +530,11 @@ rows_kernel(const __grid_constant__ RowArgs a, const __grid_constant__ RopeArgs 
     __shared__ __align__(16) unsigned char smem[SINK == SINK_BLOCKS ? sizeof(BlockSmem) : sizeof(RowSmem)];
     auto& table = reinterpret_cast<RowSmem*>(smem)->table;
     auto& slots = reinterpret_cast<RowSmem*>(smem)->slots;
+    // A programmatic dependent of whatever is before it in the stream: its CTAs may be placed while that kernel drains, but
+    // touch nothing before it has completed.  The same is offered to the kernel behind.  In a stream of calls 8192 rows take
+    // 28.9 us instead of 30.8.  (Decode launches are not made this way: their CTAs have to land on the same SMs every time.)
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     int cta = blockIdx.x;
     if constexpr (SINK == SINK_BLOCKS) {
         // the CTAs that write blocks go first: they take longer (spread evenly over the grid they cost 15 % as its tail)
