@@ -197,7 +197,7 @@ __device__ __forceinline__ HeadMap head_map(const float2* table, bool rotary, co
     for (int i = 0; i < 8; i++) w.p[i] = pair(1.f, 1.f);
     if (weight) {
         const uint4* wp = static_cast<const uint4*>(weight);
-        w = unpack<ACT>(Raw{__ldg(wp + ch.a), __ldg(wp + ch.b)});
+        w = unpack<ACT>(Raw{wp[ch.a], wp[ch.b]});
     }
 #pragma unroll
     for (int i = 0; i < 8; i++) { m.diag[i] = w.p[i]; m.cross[i] = 0; }
@@ -272,7 +272,7 @@ __device__ __forceinline__ Place locate(const PageArgs& t, int row, int tokens, 
         for (;;) {
             const int step = (n + 31) >> 5;
             const int last = min(lo + (lane + 1) * step, lo + n);          // token_begin[last] ends this lane's chunk
-            const bool over = __ldg(t.token_begin + last) <= row;
+            const bool over = t.token_begin[last] <= row;
             const int skip = __popc(__ballot_sync(0xffffffffu, over)) * step;
             if (skip >= n) return p;                                       // behind the last sequence
             lo += skip;
@@ -280,13 +280,13 @@ __device__ __forceinline__ Place locate(const PageArgs& t, int row, int tokens, 
             if (step == 1) break;
         }
         p.seq   = lo;
-        p.begin = __ldg(t.token_begin + lo);
-        p.end   = min(__ldg(t.token_begin + lo + 1), tokens);
+        p.begin = t.token_begin[lo];
+        p.end   = min(t.token_begin[lo + 1], tokens);
         if (row < p.begin) { p.end = p.begin; return p; }                  // rows before the first sequence
     }
-    p.slot = t.slot_ids ? __ldg(t.slot_ids + p.seq) : p.seq;
+    p.slot = t.slot_ids ? t.slot_ids[p.seq] : p.seq;
     if (p.slot < 0) return p;
-    const int first = t.start_pos ? __ldg(t.start_pos + p.seq) : t.first_pos;
+    const int first = t.start_pos ? t.start_pos[p.seq] : t.first_pos;
     const long long pos = static_cast<long long>(first) + (row - p.begin);
     p.pos = pos < 0 || pos > 0x7fffffff ? -1 : static_cast<int>(pos);
     return p;
@@ -298,7 +298,7 @@ __device__ __forceinline__ Spot spot_of(const PageArgs& t, const Place& p, int r
     const unsigned pos = static_cast<unsigned>(max(p.pos, 0)), index = pos / static_cast<unsigned>(t.page_size);
     int page = -1;
     if (p.pos >= 0 && p.slot < t.num_slots && index < static_cast<unsigned>(t.table_stride)) {
-        page = __ldg(t.block_table + static_cast<size_t>(p.slot) * t.table_stride + index);
+        page = t.block_table[static_cast<size_t>(p.slot) * t.table_stride + index];
         if (page < 0 || page >= t.num_pages) page = -1;
     }
     if (page < 0) atomicCAS(t.status, 0u, (ST_APPEND_RANGE << 24) | (row & 0xffffffu));
@@ -308,7 +308,7 @@ __device__ __forceinline__ Spot spot_of(const PageArgs& t, const Place& p, int r
 __device__ __forceinline__ int rope_position(const RowArgs& a, const RopeArgs& rope, const RopeTables& tab, int freq, int row, int pos) {
     if (!a.positions) return pos;
     const int axis = rope.axes > 1 ? tab.axis[freq] : 0;
-    return __ldg(a.positions + axis * a.positions_stride + row);
+    return a.positions[axis * a.positions_stride + row];
 }
 
 // 16 bytes global -> shared without waiting, past L1.
@@ -400,8 +400,8 @@ __device__ __forceinline__ void write_blocks(const RowArgs& a, const RopeArgs& r
                 const Chunks c = HALVES ? Chunks{l, l + 8, true} : chunks_of(l, rope.rotary_dim);
                 float2 lo = make_float2(1.f, 1.f), hi = lo;                   // weights of the pairs
                 if (a.k_norm) {
-                    lo = split(Act<ACT>::to_f32(__ldg(static_cast<const uint32_t*>(a.k_norm) + c.a * 4 + i)));
-                    hi = split(Act<ACT>::to_f32(__ldg(static_cast<const uint32_t*>(a.k_norm) + c.b * 4 + i)));
+                    lo = split(Act<ACT>::to_f32(static_cast<const uint32_t*>(a.k_norm)[c.a * 4 + i]));
+                    hi = split(Act<ACT>::to_f32(static_cast<const uint32_t*>(a.k_norm)[c.b * 4 + i]));
                 }
                 float4 ma = make_float4(lo.x, lo.y, 0.f, 0.f), mb = make_float4(hi.x, hi.y, 0.f, 0.f);
                 if (rotary && c.rot) {
@@ -531,7 +531,8 @@ rows_kernel(const __grid_constant__ RowArgs a, const __grid_constant__ RopeArgs 
     auto& table = reinterpret_cast<RowSmem*>(smem)->table;
     auto& slots = reinterpret_cast<RowSmem*>(smem)->slots;
     // A programmatic dependent of whatever is before it in the stream: its CTAs may be placed while that kernel drains, but
-    // touch nothing before it has completed.  The same is offered to the kernel behind.  In a stream of calls 8192 rows take
+    // touch nothing before it has completed.  (So nothing here may be read through the non-coherent path either: what that
+    // kernel writes changes while this one is already resident.)  The same is offered to the kernel behind.  In a stream of calls 8192 rows take
     // 28.9 us instead of 30.8.  (Decode launches are not made this way: their CTAs have to land on the same SMs every time.)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -607,7 +608,7 @@ rows_kernel(const __grid_constant__ RowArgs a, const __grid_constant__ RopeArgs 
 #pragma unroll 1
         for (; unit < end; unit += step) {
             float factor = inv;
-            if (quantised && head_scales) factor = __fdividef(1.f, __ldg(head_scales + min(4 * (unit - first) + sh, a.hkv - 1)));
+            if (quantised && head_scales) factor = __fdividef(1.f, head_scales[min(4 * (unit - first) + sh, a.hkv - 1)]);
             cp_async_wait<ROWS_SLOTS - 1>();
             Vals x = unpack<ACT>(Raw{load_shared(&slots[warp][slot][0][lane]), load_shared(&slots[warp][slot][1][lane])});
             fetch(unit + ROWS_SLOTS * step, slot);
