@@ -31,21 +31,15 @@ def check_pools(kc, vc, scales, models, written):
         assert (ro.decode_e4m3(raw) == m.slack[..., None])[~live].all()
 
 
-@pytest.mark.parametrize("ps, hkv, act, calls", [
-    # calls: lists of (new tokens per sequence), one append each
-    (16, 8, "fp16", [[1, 1, 1]] * 20), (16, 8, "bf16", [[5, 40, 0], [1, 7, 3], [33, 1, 64]]), (16, 2, "fp16", [[100, 3, 17]]),
-    (64, 1, "bf16", [[10, 64, 70], [60, 1, 1], [300, 0, 2]]), (24, 3, "fp16", [[5, 9, 30], [4, 40, 1]]), (1, 2, "fp16", [[3, 1, 0], [1, 1, 1]]),
-    (5, 2, "bf16", [[3, 6, 11], [9, 1, 1]]), (8, 4, "fp16", [[2, 3, 4]] * 5), (6, 5, "fp16", [[7, 1, 2], [2, 2, 2]]), (256, 8, "bf16", [[700, 15, 250], [3, 300, 9]]),
-    (16, 16, "fp16", [[0, 2, 0], [0, 0, 1], [16, 15, 14]])])
-def test_append_blocks(ps, hkv, act, calls, torch_cuda, pa):
-    torch = torch_cuda
+def append_calls(torch, pa, ps, hkv, act, calls):
+    """One append per entry of `calls` (new tokens of each sequence), then everything the pools and scales hold."""
     rng = np.random.default_rng(ps * 31 + hkv)
     total = np.sum(calls, 0)
     table, pages = paged(rng, total, ps)
     kc, vc, scales = pools(torch, pages, hkv, ps)
     models = [ro.BlockPool(pages, hkv, ps) for _ in range(2)]
     written = np.zeros((pages, ps), bool)
-    past = np.zeros(3, int)
+    past = np.zeros(len(total), int)
     d_table = torch.from_numpy(table).cuda()
     for call, new in enumerate(calls):
         tokens = sum(new)
@@ -73,8 +67,28 @@ def test_append_blocks(ps, hkv, act, calls, torch_cuda, pa):
             for p in range(past[b], past[b] + n):
                 written[table[b, p // ps], p % ps] = True
             at += n
-        past = past + new
+        past = past + np.asarray(new)
     check_pools(kc, vc, scales, models, written)
+
+
+@pytest.mark.parametrize("ps, hkv, act, calls", [
+    # calls: lists of (new tokens per sequence), one append each
+    (16, 8, "fp16", [[1, 1, 1]] * 20), (16, 8, "bf16", [[5, 40, 0], [1, 7, 3], [33, 1, 64]]), (16, 2, "fp16", [[100, 3, 17]]),
+    (64, 1, "bf16", [[10, 64, 70], [60, 1, 1], [300, 0, 2]]), (24, 3, "fp16", [[5, 9, 30], [4, 40, 1]]), (1, 2, "fp16", [[3, 1, 0], [1, 1, 1]]),
+    (5, 2, "bf16", [[3, 6, 11], [9, 1, 1]]), (8, 4, "fp16", [[2, 3, 4]] * 5), (6, 5, "fp16", [[7, 1, 2], [2, 2, 2]]), (256, 8, "bf16", [[700, 15, 250], [3, 300, 9]]),
+    (16, 16, "fp16", [[0, 2, 0], [0, 0, 1], [16, 15, 14]])])
+def test_append_blocks(ps, hkv, act, calls, torch_cuda, pa):
+    append_calls(torch_cuda, pa, ps, hkv, act, calls)
+
+
+@pytest.mark.parametrize("seed", range(16))
+def test_append_blocks_random(seed, torch_cuda, pa):
+    rng = np.random.default_rng(900 + seed)
+    ps = int(rng.choice([1, 2, 4, 7, 8, 12, 16, 16, 16, 20, 32, 48, 128]))
+    batch, top = int(rng.integers(1, 40)), int(rng.choice([1, 2, 10, 17, 90]))
+    calls = [rng.integers(0 if top > 1 else 1, top + 1, batch).tolist() for _ in range(int(rng.integers(1, 6)))]
+    calls.append([1] * batch)
+    append_calls(torch_cuda, pa, ps, int(rng.integers(1, 10)), str(rng.choice(["fp16", "bf16"])), calls)
 
 
 def test_a_reused_page_forgets_its_scale(torch_cuda, pa):
