@@ -1781,6 +1781,8 @@ int append_batch_impl(pd_cache* c, int count, const int* slots, const void* cons
         units += static_cast<long long>(n[i]) * c->cfg.num_kv_heads * 16;
     }
     if (as_rows) begin[count] = token;
+    // the previous batch's kernels, perhaps on another stream, still read the device copy of their lists
+    if (c->batch_pending) PD_CUDA(cudaStreamWaitEvent(stream, c->batch_done, 0));
     PD_CUDA(cudaMemcpyAsync(c->batch_device, c->batch_staging, total, cudaMemcpyHostToDevice, stream));
     PD_CUDA(cudaEventRecord(c->batch_staged, stream));
     char* d = static_cast<char*>(c->batch_device);

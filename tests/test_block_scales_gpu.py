@@ -498,3 +498,38 @@ def test_params_of_a_block_scaled_cache_do_not_fit_another_decode(torch_cuda, pa
     assert c.params().k_scale == 1.0
     c.set_block_scales()
     assert np.isnan(c.params().k_scale) and np.isnan(c.params().v_scale)
+
+
+@pytest.mark.parametrize("blocks", [False, True])
+def test_batches_on_alternating_streams(blocks, torch_cuda, pa):
+    """Appends to one cache from two streams in turn, nothing waited for: each batch's lists are its own."""
+    torch = torch_cuda
+    hkv, slots, steps = 2, 24, 30
+    c = pa.PagedKVCache(pa.PagedKVCache.Config(slots * 4, 16, hkv, 128, slots, 4, pa.KVDtype.FP8_E4M3 if blocks else pa.KVDtype.FP16))
+    if blocks:
+        c.set_block_scales()
+    ids = [c.admit() for _ in range(slots)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    # token i of a slot is 2^(i % 5) everywhere: exact in every type and under every block's scale
+    inputs = []
+    for i in range(steps):
+        x = torch.full((slots, hkv, 128), float(2 ** (i % 5)), dtype=torch.float16, device="cuda")
+        inputs.append((x, pa.qkv_params(None, x, x)))
+    torch.cuda.synchronize()
+    for i, (x, p) in enumerate(inputs):
+        order = ids if i % 3 else ids[::-1]
+        assert c.append_qkv(order, [1] * slots, p, None, None, streams[i % 2].cuda_stream)
+    torch.cuda.synchronize()
+    assert pa.kernel_status() == 0
+    prm = c.params()
+    raw = device_view(prm.k_cache, slots * 4 * hkv * 16 * 128 * (1 if blocks else 2), torch).cpu().numpy()
+    val = ro.decode_e4m3(raw) if blocks else raw.view(np.float16).astype(np.float64)
+    val = val.reshape(slots * 4, hkv, 16, 128)
+    if blocks:
+        sc = device_view(c.block_scales(), slots * 4 * hkv * 8, torch).cpu().numpy().view(np.float32).reshape(slots * 4, hkv, 1, 2)
+        val = val * sc[..., 0, None]
+    want = 2.0 ** (np.arange(steps) % 5)
+    for s in ids:
+        at = np.arange(steps)
+        got = val[c.block_table(s)[at // 16], :, at % 16]
+        assert np.array_equal(got, np.broadcast_to(want[:, None, None], got.shape))
