@@ -253,6 +253,20 @@ __device__ __forceinline__ float inv_rms(const Vals& x, float eps) {
     return rsqrtf(ss * (1.f / 128.f) + eps);
 }
 
+// What a kernel of this library may just have written - rows, scales, bytes of the pool - is read past L1: the kernel before may
+// have brought older lines into the SM's L1 while this grid was already waiting for it (see rows_kernel).  Lists, positions
+// and weights come from elsewhere and may use L1; nothing uses the non-coherent path.
+__device__ __forceinline__ float load_float(const float* p) {
+    float v;
+    asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint4 load_16(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.cg.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+    return v;
+}
+
 // The sequence a row belongs to and its place there.  Called by whole warps; every lane gets the answer.
 struct Place {
     int seq, slot;      // slot < 0: the row belongs to no sequence, or to a skipped one
@@ -390,8 +404,14 @@ __device__ __forceinline__ void write_blocks(const RowArgs& a, const RopeArgs& r
             }
             cp_async_commit();
         };
+        // the scale of a begun block, asked for a unit ahead like its rows
+        auto begun_scale = [&](int u) {
+            const bool is_v = u >= a.hkv;
+            return inside && u < 2 * a.hkv ? load_float(scales + (is_v ? u - a.hkv : u) * 2 * per_page + is_v) : 0.f;
+        };
         int u = share * teams + team, slot = 0;
         fetch(u, 0);
+        float next = begun_scale(u);
         if (mapped) {
             __syncthreads();                                                  // the previous block's map has been read
             const RopeTables tab = rope_tables(rope);
@@ -428,8 +448,9 @@ __device__ __forceinline__ void write_blocks(const RowArgs& a, const RopeArgs& r
             for (; u < end; u += step) {
                 const int h = is_v ? u - a.hkv : u;
                 float* scale_at = scales + h * 2 * per_page + is_v;
-                float old = inside ? *scale_at : 0.f;
+                float old = next;
                 fetch(u + step, slot ^ 1);
+                next = begun_scale(u + step);
                 cp_async_wait<1>();
                 Vals x[2];
                 float top = 0.f;
@@ -494,7 +515,7 @@ __device__ __forceinline__ void write_blocks(const RowArgs& a, const RopeArgs& r
                     for (int r = mine; r < (paired ? min(block, 8 * half + 8) : block); r += 4) {
                         if (r >= inside && r < inside + n) continue;          // just written
                         uint4* at = reinterpret_cast<uint4*>(was + r * 128) + j;
-                        const uint4 b = *at;
+                        const uint4 b = load_16(at);
                         const uint32_t in[4] = {b.x, b.y, b.z, b.w};
                         uint32_t out[4];
 #pragma unroll
@@ -531,8 +552,7 @@ rows_kernel(const __grid_constant__ RowArgs a, const __grid_constant__ RopeArgs 
     auto& table = reinterpret_cast<RowSmem*>(smem)->table;
     auto& slots = reinterpret_cast<RowSmem*>(smem)->slots;
     // A programmatic dependent of whatever is before it in the stream: its CTAs may be placed while that kernel drains, but
-    // touch nothing before it has completed.  (So nothing here may be read through the non-coherent path either: what that
-    // kernel writes changes while this one is already resident.)  The same is offered to the kernel behind.  In a stream of calls 8192 rows take
+    // touch nothing before it has completed.  The same is offered to the kernel behind.  In a stream of calls 8192 rows take
     // 28.9 us instead of 30.8.  (Decode launches are not made this way: their CTAs have to land on the same SMs every time.)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");

@@ -533,3 +533,40 @@ def test_batches_on_alternating_streams(blocks, torch_cuda, pa):
         at = np.arange(steps)
         got = val[c.block_table(s)[at // 16], :, at % 16]
         assert np.array_equal(got, np.broadcast_to(want[:, None, None], got.shape))
+
+
+def test_calls_right_behind_one_another(torch_cuda, pa):
+    """Each call reads what the one before it wrote - rows rotated in place, a block's scale and bytes, positions - with nothing
+    in between; the same sequence with waits in between must leave the same bits."""
+    torch = torch_cuda
+    hq, hkv, batch, steps = 4, 2, 96, 48
+    rng = np.random.default_rng(3)
+    rows = torch.from_numpy(rng.standard_normal((steps, batch, hq + 2 * hkv, 128)) * 2.0 ** rng.integers(-5, 6, (steps, batch, 1, 1))).half().cuda()
+    w = torch.rand(128, device="cuda").add_(0.5).half()
+    rope = pa.Rope.with_base()
+    results = []
+    for wait in (True, False):
+        x = rows.clone()
+        kc, vc, scales = pools(torch, batch * 3, hkv, 16)
+        table = torch.arange(batch * 3, dtype=torch.int32, device="cuda").view(batch, 3)
+        starts = torch.arange(steps, dtype=torch.int32, device="cuda")[:, None].expand(steps, batch).contiguous()
+        q = torch.zeros(steps, batch, hq, 128, dtype=torch.float16, device="cuda")
+        calls = []
+        for i in range(steps):
+            r = x[i]
+            first = pa.qkv_params(r[:, :hq], r[:, hq:hq + hkv], r[:, hq + hkv:], q_norm=w, k_norm=w, positions=starts[i])
+            plain = pa.qkv_params(r[:, :hq], r[:, hq:hq + hkv], r[:, hq + hkv:])
+            calls.append((first, plain, r, pa.append_target(kc, vc, table, starts[i], d_block_scales=scales)))
+        torch.cuda.synchronize()
+        for i, (first, plain, r, target) in enumerate(calls):
+            pa.qk_norm_rope(first, rope, r[:, :hq], r[:, hq:hq + hkv])
+            if wait:
+                torch.cuda.synchronize()
+            pa.append_qkv(FP8, plain, None, target, q[i])
+            if wait:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        results.append((x, kc, vc, scales, q))
+    assert pa.kernel_status() == 0
+    for a, b in zip(*results):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
