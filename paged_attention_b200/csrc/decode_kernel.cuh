@@ -869,6 +869,7 @@ paged_decode_kernel(const __grid_constant__ pd_params p, const __grid_constant__
             }
             seg = n_seg; sg = n_sg; bt = n_bt; tok = n_tok; page = n_page;
         }
+        if constexpr (BS) asm volatile("cp.async.wait_all;" ::: "memory");   // no lane leaves with scales of its own on their way
         if (!ok || *abort_flag) {
             // Drain: no copy may still be in flight towards this CTA's shared memory at exit.
             for (int i = 0; i < min(issued, nst); i++) {
