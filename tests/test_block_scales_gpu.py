@@ -570,3 +570,28 @@ def test_calls_right_behind_one_another(torch_cuda, pa):
     assert pa.kernel_status() == 0
     for a, b in zip(*results):
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+def test_a_pool_past_32_bits(torch_cuda, pa):
+    """Appends to and decode from the far end of pools of more than 2^32 bytes."""
+    torch = torch_cuda
+    hq, hkv, ps, pages, n = 16, 8, 16, 280000, 100           # 280000 * 8 * 16 * 128 = 4.6 GB
+    kc, vc = (torch.zeros(pages, hkv, ps, 128, dtype=torch.uint8, device="cuda") for _ in range(2))
+    scales = torch.zeros(pages, hkv, 1, 2, device="cuda")
+    ids = [pages - 1 - 3 * i for i in range(7)]
+    table = torch.tensor([ids], dtype=torch.int32, device="cuda")
+    w = Rows(torch, pa, n, hq, hkv, seed=4)
+    q = torch.zeros(n, hq, 128, dtype=torch.float16, device="cuda")
+    start, begin = torch.zeros(1, dtype=torch.int32, device="cuda"), torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    pa.append_qkv(FP8, w.params(), w.rope, pa.append_target(kc, vc, table, start, begin, d_block_scales=scales), q)
+    dq, lens = q[-1:].contiguous(), torch.tensor([n], dtype=torch.int32, device="cuda")
+    out = torch.zeros_like(dq)
+    p, dp = bind(torch, pa, dq, out, kc, vc, table, lens, [n], hq, hkv, ps)
+    pa.paged_decode(FP8, p, 0, pages, d_block_scales=scales)
+    assert pa.kernel_status() == 0
+    near = [x[torch.tensor(ids, device="cuda")].cpu().numpy() for x in (kc, vc, scales)]
+    want, tol = want_decode(dq.cpu().numpy(), near[:2], near[2], np.arange(7, dtype=np.int32)[None], [n], ps)
+    assert (np.abs(out.double().cpu().numpy() - want) <= tol).all() and np.abs(want).max() > 0.1
+    k = w.want(w.k, w.wk, np.arange(n))[0]
+    got = (ro.decode_e4m3(near[0]) * near[2][..., 0, None])[np.arange(n) // ps, :, np.arange(n) % ps]
+    assert (np.abs(got - k) <= 1.1 * np.abs(k) * 2.0 ** -4 + np.abs(k).max() * 2.0 ** -15).all()

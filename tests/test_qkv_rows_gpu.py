@@ -300,3 +300,86 @@ def test_tensors_of_another_device_are_refused(torch_cuda, pa):
     x._device = 5                                   # as a tensor on cuda:5 would say
     with pytest.raises(pa.InvalidArgument, match="current device"):
         pa.qk_norm_rope(x, w.rope, torch.zeros_like(w.q), torch.zeros_like(w.k))
+
+
+@pytest.mark.parametrize("blocks", [False, True])
+@pytest.mark.parametrize("axes, r, interleaved", [(1, 128, False), (3, 128, False), (4, 96, True), (2, 16, False)])
+def test_append_with_positions_of_its_own(blocks, axes, r, interleaved, torch_cuda, pa):
+    """Rotation positions that are not the places in the cache (offsets, several axes, negative and far ones)."""
+    torch = torch_cuda
+    new, past, ps, hkv = [20, 1, 7, 16], [5, 0, 31, 16], 16, 3
+    rng = np.random.default_rng(axes)
+    table, pages = paged(rng, [a + b for a, b in zip(new, past)], ps)
+    tokens = sum(new)
+    pos = rng.integers(-10 ** 6, 10 ** 9, (axes, tokens))
+    w = Rows(torch, pa, tokens, 6, hkv, act="bf16", r=r, interleaved=interleaved, axes=axes, positions=pos)
+    kc, vc = (torch.zeros(pages, hkv, ps, 128, dtype=torch.uint8 if blocks else torch.float16, device="cuda") for _ in range(2))
+    scales = torch.zeros(pages, hkv, 1, 2, device="cuda") if blocks else None
+    q_out = torch.zeros(tokens, 6, 128, dtype=torch.float16, device="cuda")
+    t = pa.append_target(kc, vc, torch.from_numpy(table).cuda(), torch.tensor(past, dtype=torch.int32, device="cuda"),
+                         torch.from_numpy(np.cumsum([0] + new).astype(np.int32)).cuda(), d_block_scales=scales)
+    pa.append_qkv(FP8 if blocks else FP16, w.params(), w.rope, t, q_out)
+    assert pa.kernel_status() == 0
+    assert_rows(q_out, *w.want(w.q, w.wq, pos), *STEP["fp16"])
+    k, size = w.want(w.k, w.wk, pos)
+    seq = np.repeat(np.arange(4), new)
+    place = np.concatenate([np.arange(o, o + n) for n, o in zip(new, past)])
+    page, off = table[seq, place // ps], place % ps
+    if blocks:
+        s = scales.cpu().numpy().astype(np.float64)[page, :, 0, 0][..., None]
+        got, bound = ro.decode_e4m3(kc.cpu().numpy())[page, :, off] * s, ro.e4m3_bound(k, s) + 1.07 * ro.rows_bound(k, size, 0, 0)
+    else:
+        got, bound = kc.double().cpu().numpy()[page, :, off], ro.rows_bound(k, size, *STEP["fp16"])
+    assert (np.abs(got - k) <= bound).all()
+
+
+def test_forty_thousand_sequences(torch_cuda, pa):
+    """The search for a row's sequence over several levels, with empty sequences between."""
+    torch = torch_cuda
+    rng = np.random.default_rng(1)
+    batch = 40000
+    new = rng.integers(0, 2, batch)
+    new[-1] = 1
+    new[:100] = 0
+    past = rng.integers(0, 12, batch)
+    tokens = int(new.sum())
+    w = Rows(torch, pa, tokens + 3, 1, 1, norm=False)
+    kc, vc = (torch.zeros(batch, 1, 16, 128, dtype=torch.float16, device="cuda") for _ in range(2))
+    table = torch.randperm(batch, device="cuda").to(torch.int32)[:, None].contiguous()
+    q_out = torch.full((tokens + 3, 1, 128), 9.0, dtype=torch.float16, device="cuda")
+    t = pa.append_target(kc, vc, table, torch.from_numpy(past.astype(np.int32)).cuda(),
+                         torch.from_numpy(np.cumsum(np.append(0, new)).astype(np.int32)).cuda())
+    pa.append_qkv(FP16, w.params(), w.rope, t, q_out)
+    assert pa.kernel_status() == 0
+    seq = np.repeat(np.arange(batch), new)
+    place = past[seq]
+    pages = table[:, 0].cpu().numpy()[seq]
+    k, size = w.want(w.k, None, np.append(place, [0, 0, 0]))
+    got = kc.double().cpu().numpy()[pages, :, place]
+    assert (np.abs(got - k[:tokens]) <= ro.rows_bound(k, size, *STEP["fp16"])[:tokens]).all()
+    assert torch.equal(vc[torch.from_numpy(pages).long().cuda(), :, torch.from_numpy(place).cuda()], w.v[:tokens])
+    assert (vc != 0).any(-1).sum() == tokens and (q_out[tokens:] == 9).all()
+
+
+def test_empty_calls_and_one_kind_of_heads(torch_cuda, pa):
+    """No tokens, no sequences, no q heads, no k heads: nothing happens where there is nothing to do."""
+    torch = torch_cuda
+    e = torch.empty(0, 4, 128, dtype=torch.float16, device="cuda")
+    pa.qk_norm_rope(pa.qkv_params(e, e[:, :2]), None, e.clone(), e[:, :2].clone())
+    kc, vc = (torch.zeros(2, 2, 16, 128, dtype=torch.float16, device="cuda") for _ in range(2))
+    table = torch.zeros(1, 2, dtype=torch.int32, device="cuda")
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    pa.append_qkv(FP16, pa.qkv_params(e, e[:, :2], e[:, :2]), None, pa.append_target(kc, vc, table, torch.zeros(1, dtype=torch.int32, device="cuda")), e.clone())
+    x = torch.ones(3, 2, 128, dtype=torch.float16, device="cuda")
+    pa.append_qkv(FP16, pa.qkv_params(None, x, x), None, pa.append_target(kc, vc, table, none), None)
+    assert not kc.any()
+    q, out = torch.randn(3, 5, 128, device="cuda").half(), torch.zeros(3, 5, 128, dtype=torch.float16, device="cuda")
+    pa.qk_norm_rope(pa.qkv_params(q, x[:, :0]), None, out, None)
+    assert torch.equal(out, q)
+    # per-head scales for K beside a per-tensor scale for V
+    k8, v8 = (torch.zeros(2, 2, 16, 128, dtype=torch.uint8, device="cuda") for _ in range(2))
+    t = pa.append_target(k8, v8, table, torch.tensor([2], dtype=torch.int32, device="cuda"), torch.tensor([0, 3], dtype=torch.int32, device="cuda"),
+                         v_scale=0.25, d_k_scales=torch.tensor([1.0, 2.0], device="cuda"))
+    pa.append_qkv(FP8, pa.qkv_params(None, x, x), None, t, None)
+    k, v = (ro.decode_e4m3(p.cpu().numpy())[0, :, 2:5] for p in (k8, v8))
+    assert (k[0] == 1).all() and (k[1] == 0.5).all() and (v == 4).all()
