@@ -1178,7 +1178,9 @@ paged_decode_kernel(const __grid_constant__ pd_params p, const __grid_constant__
 // ROW_ITEMS = true: the plan's work items are rows (head-fused tiles).
 constexpr int MERGE_WIDE_MIN = 8;
 // One (row, query head) pair by the four warps of a CTA; s0, s1: the pair's segment range.
-template<int GROUP, bool ROW_ITEMS>
+// WARPS, LOADS: warps of the CTA and pieces each has in flight.  The block-scaled decode takes 16 warps with four pieces each
+// while that many warps fit at once (a merge of 71 pieces is two rounds of loads instead of five).
+template<int GROUP, bool ROW_ITEMS, int WARPS = 4>
 __device__ __forceinline__ void merge_pair(const pd_params& p, int idx, int s0, int s1, int seg_limit, float4 (*part_num)[32], float* part_den)
 {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -1199,12 +1201,12 @@ __device__ __forceinline__ void merge_pair(const pd_params& p, int idx, int s0, 
     for (int o = 16; o > 0; o >>= 1) lse_max = fmaxf(lse_max, __shfl_xor_sync(0xffffffffu, lse_max, o));
     float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
     float den = 0.f;
-    for (int base = s0 + warp; base < s1; base += 16) {
+    for (int base = s0 + warp; base < s1; base += 4 * WARPS) {
         float  w[4];
         float4 o[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const int s = base + 4 * j;
+            const int s = base + WARPS * j;
             const bool live = s < s1;
             w[j] = live ? exp2f(__ldcg(p.partial_lse + s * stride + gq) - lse_max) : 0.f;
             o[j] = live ? __ldcg(reinterpret_cast<const float4*>(
@@ -1223,7 +1225,7 @@ __device__ __forceinline__ void merge_pair(const pd_params& p, int idx, int s0, 
     __syncthreads();
     if (warp != 0) return;
 #pragma unroll
-    for (int w = 1; w < 4; w++) {
+    for (int w = 1; w < WARPS; w++) {
         const float4 other = part_num[w][lane];
         num.x += other.x; num.y += other.y; num.z += other.z; num.w += other.w;
         den += part_den[w];
@@ -1239,12 +1241,12 @@ __device__ __forceinline__ void merge_pair(const pd_params& p, int idx, int s0, 
 // WALK = false: one CTA per pair (grid = pairs).  WALK = true: a capped grid whose CTAs walk their pairs;
 // used when there are thousands of pairs, which is where this kernel is launched although almost every
 // pair is done after reading two integers (plans cut on the device).
-template<int GROUP, bool ROW_ITEMS = false, bool WALK = false>
-__global__ void __launch_bounds__(128)
+template<int GROUP, bool ROW_ITEMS = false, bool WALK = false, int WARPS = 4>
+__global__ void __launch_bounds__(WARPS * 32)
 merge_segments_kernel(const __grid_constant__ pd_params p, const int seg_limit)
 {
-    __shared__ float4 part_num[4][32];
-    __shared__ float  part_den[4];
+    __shared__ float4 part_num[WARPS][32];
+    __shared__ float  part_den[WARPS];
     const int pairs = p.batch * p.num_q_heads;
     auto item_of = [&](int idx) {
         const int b = idx / p.num_q_heads, hq = idx % p.num_q_heads;
@@ -1260,11 +1262,11 @@ merge_segments_kernel(const __grid_constant__ pd_params p, const int seg_limit)
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (static_cast<int>(blockIdx.x) >= pairs) return;
-    merge_pair<GROUP, ROW_ITEMS>(p, blockIdx.x, s0, s1, seg_limit, part_num, part_den);
+    merge_pair<GROUP, ROW_ITEMS, WARPS>(p, blockIdx.x, s0, s1, seg_limit, part_num, part_den);
     if constexpr (WALK) {
         for (int idx = blockIdx.x + gridDim.x; idx < pairs; idx += gridDim.x) {
             __syncthreads();   // the scratch is reused
-            merge_pair<GROUP, ROW_ITEMS>(p, idx, p.item_seg_begin[item_of(idx)], p.item_seg_begin[item_of(idx) + 1],
+            merge_pair<GROUP, ROW_ITEMS, WARPS>(p, idx, p.item_seg_begin[item_of(idx)], p.item_seg_begin[item_of(idx) + 1],
                                          seg_limit, part_num, part_den);
         }
     }

@@ -76,7 +76,7 @@ struct KernelInfo {
     int tile, threads, smem, per_sm, stages;
     void (*launch)(const pd_params&, const CUtensorMap&, const CUtensorMap&, int, int, int, unsigned*, const pdk::GatherOut&,
                    const pdk::HeadScales&, const pdk::CtaStats&, const pdk::BlockScales&, cudaStream_t);
-    void (*merge)(const pd_params&, int, cudaStream_t);
+    void (*merge)(const pd_params&, int, bool, cudaStream_t);   // bool: of a block-scaled decode
     // the same shape over a block-scaled cache (e4m3 only): launched where BlockScales carries an array
     const void* scaled_fn;
     int scaled_smem;               // with one scale per token, the most it can need
@@ -106,10 +106,10 @@ const void* scaled_kernel() {
 // complete, which takes the launch latency out of the gap between the two kernels.
 constexpr int MERGE_GRID_CAP = 148 * 8;
 template<typename Kernel>
-void launch_dependent(Kernel kernel, int blocks, const pd_params& p, int seg_limit, cudaStream_t stream) {
+void launch_dependent(Kernel kernel, int blocks, const pd_params& p, int seg_limit, cudaStream_t stream, int threads = 128) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(blocks));
-    cfg.blockDim = dim3(128);
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
     cfg.stream = stream;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -118,10 +118,15 @@ void launch_dependent(Kernel kernel, int blocks, const pd_params& p, int seg_lim
     cfg.numAttrs = 1;
     cudaLaunchKernelEx(&cfg, kernel, p, seg_limit);
 }
+// A block-scaled decode of few (row, head) pairs, and so of many pieces each, merges them with 16 warps per pair: two such
+// CTAs fit on an SM.
+constexpr int WIDE_MERGE_PAIRS = 148 * 2, WIDE_MERGE_WARPS = 16;
 template<int GROUP>
-void launch_merge(const pd_params& p, int seg_limit, cudaStream_t stream) {
+void launch_merge(const pd_params& p, int seg_limit, bool scaled, cudaStream_t stream) {
     const int pairs = p.batch * p.num_q_heads;
-    if (pairs > MERGE_GRID_CAP) launch_dependent(pdk::merge_segments_kernel<GROUP, false, true>, MERGE_GRID_CAP, p, seg_limit, stream);
+    if (scaled && pairs <= WIDE_MERGE_PAIRS)
+        launch_dependent(pdk::merge_segments_kernel<GROUP, false, false, WIDE_MERGE_WARPS>, pairs, p, seg_limit, stream, 32 * WIDE_MERGE_WARPS);
+    else if (pairs > MERGE_GRID_CAP) launch_dependent(pdk::merge_segments_kernel<GROUP, false, true>, MERGE_GRID_CAP, p, seg_limit, stream);
     else                        launch_dependent(pdk::merge_segments_kernel<GROUP, false, false>, pairs, p, seg_limit, stream);
 }
 
@@ -158,7 +163,7 @@ template<> struct FusedConfig<__half> { using type = pdk::Config<8, 1, 3, 1, 8>;
 template<> struct FusedConfig<__nv_fp8_e4m3> { using type = pdk::Config<8, 2, 3, 1, 8>; };
 
 template<int GROUP>
-void launch_merge_rows(const pd_params& p, int seg_limit, cudaStream_t stream) {
+void launch_merge_rows(const pd_params& p, int seg_limit, bool, cudaStream_t stream) {
     const int pairs = p.batch * p.num_q_heads;
     if (pairs > MERGE_GRID_CAP) launch_dependent(pdk::merge_segments_kernel<GROUP, true, true>, MERGE_GRID_CAP, p, seg_limit, stream);
     else                        launch_dependent(pdk::merge_segments_kernel<GROUP, true, false>, pairs, p, seg_limit, stream);
@@ -1126,7 +1131,7 @@ int decode_impl(int dtype, const pd_params* p, int num_pages, const pdk::GatherO
     k->launch(*p, k_map, v_map, btl, row_gather ? 1 : 0, 0, status, gather, scales, pdk::CtaStats{stats_slots}, blocks, stream);
     PD_CUDA(cudaGetLastError());
     if (p->needs_merge && p->needs_merge != pdk::MERGE_IN_KERNEL) {
-        k->merge(*p, 0, stream);
+        k->merge(*p, 0, block_scales != nullptr, stream);
         PD_CUDA(cudaGetLastError());
     }
     return PD_OK;
@@ -1276,7 +1281,7 @@ int pd_paged_decode_static(int dtype, const pd_params* p, int num_segments, int 
               pdk::HeadScales{nullptr, nullptr}, pdk::CtaStats{nullptr}, pdk::BlockScales{nullptr, 0, 0}, stream);
     PD_CUDA(cudaGetLastError());
     if (local.needs_merge) {
-        k->merge(local, seg_limit, stream);
+        k->merge(local, seg_limit, false, stream);
         PD_CUDA(cudaGetLastError());
     }
     return PD_OK;
