@@ -82,9 +82,11 @@ struct HeadScales {
 // power of two of tokens that divides the page size, at most 16.  The producer warp brings a tile's pairs into the
 // tile's stage with 8-byte asynchronous copies that arrive on the same barrier as the tile: 8 bytes beside 4 KB of K and V per
 // 16 tokens and head.  Against the same decode with one scale per tensor, measured on B200: 128 x 4096 tokens 163.6 us and
-// 162.1, a ragged 256 x 4100 (64 query heads) 333.8 and 329.2 (both at the copy rate of the traffic); steps too short to be
-// bound by memory pay more for the work per tile: 16 x 4096 with groups of 8 32.4 us and 31.0, 32 x 1024 with 4 kv heads 12.9 and
-// 12.1.  Fetching the scales ahead of the products, or cheaper reciprocals, changed none of these by more than 1 %.
+// 162.1, a ragged 256 x 4100 (64 query heads) 333.8 and 329.2 (both at the copy rate of the traffic).  Steps on the
+// (row, kv head) schedule, whose warps have less time per byte, pay more: 16 x 4096 with groups of 8 32.4 us and 31.0, 32 x 1024
+// with 4 kv heads 12.9 and 12.1, 4 x 30000 with 8 kv heads 47.4 and 42.3, 1 x 200001 in pages of 64 39.7 and 39.6.  Of the 5 us
+// of 4 x 30000 half go away with constant scales that nobody loads, so half is arithmetic.  Without gain: fetching the scales
+// ahead of the products, cheaper reciprocals, prefetches into L2, plain loads by the producer's lanes one tile or four tiles ahead.
 struct BlockScales {
     const float2* scales;
     int log2_block;
