@@ -232,7 +232,8 @@ int pd_paged_decode_block_scaled(int dtype, const pd_params* p, int num_pages, c
  * 2 the caller's plan cut in unequal shares by the adaptive cut), out[1] grid, out[2] tokens per tile,
  * out[3] kv heads per tile, out[4] consumer warps per CTA, out[5] pipeline stages, out[6] CTAs per SM the
  * shape is made for, out[7] needs_merge of that schedule (0 none, 1 merge kernel, 2 merged inside the decode
- * kernel, 3 per row).  Pure host lookup; launches nothing. */
+ * kernel, 3 per row).  Pure host lookup; launches nothing.  (A block-scaled decode runs the head-fused schedule for
+ * fewer rows; pd_cache_describe_launch knows whether the cache is block-scaled.) */
 int pd_describe_launch(int dtype, const pd_params* p, int* out);
 
 /* No counterpart in the reference (its DevicePlan always allocates, src/decode/decode.cu:131-141).

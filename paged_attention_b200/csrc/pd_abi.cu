@@ -347,6 +347,8 @@ struct pd_device_plan {
     struct Fused {                 // the same step cut into head-fused row segments (valid: exactly 8 kv heads)
         bool valid = false;
         int dtype = -1, group = 0, batch = 0, num_ctas = 0, num_segments = 0, needs_merge = 0;
+        int most_pieces = 0;       // of any row, and tiles of all rows: host plans only
+        long long tiles = 0;
         size_t rows = 0;           // segments * num_q_heads
         const void* segments = nullptr;
         const int* cta_seg_begin = nullptr;
@@ -794,6 +796,9 @@ int pd_device_plan_upload(pd_device_plan* dp, const pd_plan* plan, int group, in
         f.num_ctas = rows_plan->num_ctas;
         f.num_segments = static_cast<int>(rows_plan->segments.size() / 4);
         f.needs_merge = plan_merge_mode(*rows_plan);
+        for (int b = 0; b < rows_plan->num_items; b++)
+            f.most_pieces = std::max(f.most_pieces, rows_plan->item_seg_begin[b + 1] - rows_plan->item_seg_begin[b]);
+        for (int len : plan->seq_lens) f.tiles += (len + fk->tile - 1) / fk->tile;
         f.stats = stats_fused;
         f.rows = frows;
         f.segments = a + std_bytes;
@@ -1049,7 +1054,13 @@ struct Selection {
     int schedule;                  // 0 the caller's plan, 1 head-fused rows, 2 the caller's plan in unequal shares
     unsigned long long* stats;
 };
-Selection select_schedule(int dtype, const pd_params* p, const KernelInfo* k, bool gathered, pd_params* scratch) {
+// scaled: a block-scaled decode.  On the (row, kv head) schedule its 8-byte loads of scales per 2 KB box cost up to 10 %, on the
+// head-fused one 1 %, so it is head-fused for fewer rows too: what it gains grows with a CTA's tiles, what the merge costs with
+// a row's pieces.  Rows cut in up to 24 pieces, and two tiles per CTA for every three pieces (16 x 10000 tokens, 10 pieces and 34
+// tiles: 62.0 us and 56.3 head-fused; 16 x 2000, 10 and 7: 19.7 and 17.8; 8 x 30000, 19 and 51: 86.7 and 81.2; 8 x 8000, 19 and 14:
+// 28.7 and 28.8; on the other side 16 x 1000, 10 and 3: 12.8 and 13.8; 4 x 30000, 37 and 25: 47.1 and 47.8).
+constexpr int SCALED_MOST_PIECES = 24;
+Selection select_schedule(int dtype, const pd_params* p, const KernelInfo* k, bool gathered, bool scaled, pd_params* scratch) {
     Selection sel{p, k, 1, 0, nullptr};
     AltSchedules alt;
     {
@@ -1065,7 +1076,9 @@ Selection select_schedule(int dtype, const pd_params* p, const KernelInfo* k, bo
     const KernelInfo* fk = p->num_kv_heads == FUSED_HEADS ? fused_info(dtype, group) : nullptr;
     // Head-fused, mode 1: not where rows would be spread over more than 4 CTAs each.
     const bool use_fused = fk && g_head_fused && matches(alt.fused) &&
-                           (g_head_fused == 2 || alt.fused.needs_merge != pdk::MERGE_SEPARATE);
+                           (g_head_fused == 2 || alt.fused.needs_merge != pdk::MERGE_SEPARATE ||
+                            (scaled && alt.fused.most_pieces <= SCALED_MOST_PIECES &&
+                             3 * alt.fused.tiles >= 2ll * alt.fused.most_pieces * alt.fused.num_ctas));
     const bool use_weighted = !use_fused && g_adaptive && matches(alt.weighted);
     if (g_adaptive && !use_fused && !use_weighted) sel.stats = alt.stats;
     if (use_fused || use_weighted) {
@@ -1105,7 +1118,7 @@ int decode_impl(int dtype, const pd_params* p, int num_pages, const pdk::GatherO
     if (reinterpret_cast<uintptr_t>(p->q) % 16 != 0 || reinterpret_cast<uintptr_t>(p->out) % 16 != 0)
         return set_error(PD_INVALID_ARGUMENT, "paged_decode: q and out must be 16-byte aligned");
     pd_params alt_params;
-    Selection sel = select_schedule(dtype, p, k, gather.world != 0, &alt_params);
+    Selection sel = select_schedule(dtype, p, k, gather.world != 0, block_scales != nullptr, &alt_params);
     p = sel.params;
     k = sel.kernel;
     const int box_heads = sel.box_heads;
@@ -1161,14 +1174,16 @@ int pd_paged_decode_block_scaled(int dtype, const pd_params* p, int num_pages, c
     return decode_impl(dtype, p, num_pages, pdk::GatherOut{}, stream, pdk::HeadScales{nullptr, nullptr}, d_block_scales);
 }
 
-int pd_describe_launch(int dtype, const pd_params* p, int* out) {
+}  // extern "C"
+namespace {
+int describe_launch(int dtype, const pd_params* p, bool scaled, int* out) {
     if (!p || !out) return set_error(PD_INVALID_ARGUMENT, "describe_launch: null argument");
     if (p->num_kv_heads <= 0 || p->num_q_heads % p->num_kv_heads != 0)
         return set_error(PD_INVALID_ARGUMENT, "num_q_heads must be a multiple of num_kv_heads");
     const KernelInfo* k;
     if (int rc = find_kernel(dtype, p->head_dim, p->num_q_heads / p->num_kv_heads, &k)) return rc;
     pd_params scratch;
-    const Selection sel = select_schedule(dtype, p, k, false, &scratch);
+    const Selection sel = select_schedule(dtype, p, k, false, scaled, &scratch);
     out[0] = sel.schedule;
     out[1] = sel.params->num_ctas;
     out[2] = sel.kernel->tile;
@@ -1179,6 +1194,10 @@ int pd_describe_launch(int dtype, const pd_params* p, int* out) {
     out[7] = sel.params->needs_merge;
     return PD_OK;
 }
+}  // namespace
+extern "C" {
+
+int pd_describe_launch(int dtype, const pd_params* p, int* out) { return describe_launch(dtype, p, false, out); }
 
 // ---- decode without any allocation -------------------------------------------------------------------------
 //
@@ -1975,7 +1994,7 @@ int pd_cache_describe_launch(const pd_cache* c, int* out) {
     p.batch = c->plan_batch;
     p.num_q_heads = c->plan_num_q_heads;
     pd_device_plan_bind(c->device_plan, &p);
-    return pd_describe_launch(c->cfg.dtype, &p, out);
+    return describe_launch(c->cfg.dtype, &p, c->d_block_scales != nullptr, out);
 }
 
 int pd_cache_set_head_scales(pd_cache* c, const float* k_scales, const float* v_scales) {

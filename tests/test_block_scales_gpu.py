@@ -595,3 +595,51 @@ def test_a_pool_past_32_bits(torch_cuda, pa):
     k = w.want(w.k, w.wk, np.arange(n))[0]
     got = (ro.decode_e4m3(near[0]) * near[2][..., 0, None])[np.arange(n) // ps, :, np.arange(n) % ps]
     assert (np.abs(got - k) <= 1.1 * np.abs(k) * 2.0 ** -4 + np.abs(k).max() * 2.0 ** -15).all()
+
+
+def test_schedule_of_few_long_rows(torch_cuda, pa):
+    """16 rows cut in about ten pieces each: head-fused over a block-scaled cache, (row, kv head) otherwise; both right."""
+    torch = torch_cuda
+    rng = np.random.default_rng(12)
+    lens = [2400 + 7 * i for i in range(16)]
+    c = pa.PagedKVCache(pa.PagedKVCache.Config(16 * 160, 16, 8, 128, 16, 160, pa.KVDtype.FP8_E4M3))
+    c.set_block_scales()
+    ids = [c.admit() for _ in lens]
+    tokens = sum(lens)
+    k, v = (torch.randn(tokens, 8, 128, device="cuda").half() for _ in range(2))
+    assert c.append_qkv(ids, lens, pa.qkv_params(None, k, v), None, None)
+    q = torch.from_numpy(rng.standard_normal((16, 16, 128)).astype(np.float16)).cuda()
+    outs = []
+    mode = pa.head_fused()
+    try:
+        for m, schedule in ((1, "head-fused rows"), (0, "caller's plan")):
+            pa.set_head_fused(m)
+            c.plan(ids, 16)
+            d = c.describe_launch()
+            assert d["schedule"] == schedule
+            out = torch.full_like(q, float("nan"))
+            c.run(q, out)
+            assert pa.kernel_status() == 0
+            outs.append(out)
+    finally:
+        pa.set_head_fused(mode)
+    p = c.params()
+    raw = [device_view(ptr, 16 * 160 * 8 * 16 * 128, torch).cpu().numpy().reshape(16 * 160, 8, 16, 128) for ptr in (p.k_cache, p.v_cache)]
+    sc = device_view(c.block_scales(), 16 * 160 * 8 * 8, torch).cpu().numpy().view(np.float32).reshape(16 * 160, 8, 1, 2)
+    for row in (0, 7, 15):
+        table = np.zeros((1, 160), np.int32)
+        t = c.block_table(row)
+        table[0, :len(t)] = t
+        want, tol = want_decode(q[row:row + 1].cpu().numpy(), raw, sc, table, lens[row:row + 1], 16)
+        for out in outs:
+            assert (np.abs(out[row].double().cpu().numpy() - want[0]) <= tol[0]).all()
+    # a per-tensor cache keeps its schedule
+    pa.set_head_fused(1)
+    plan = pa.make_plan(FP8, lens, 16, 8, 128)
+    dp = pa.DevicePlan()
+    dp.upload(plan, 2, 128)
+    prm = pa.DecodeParams()
+    prm.batch, prm.num_q_heads, prm.num_kv_heads, prm.head_dim, prm.page_size = 16, 16, 8, 128, 16
+    dp.bind(prm)
+    assert pa.describe_launch(FP8, prm)["schedule"] == "caller's plan"
+    pa.set_head_fused(mode)
