@@ -444,18 +444,31 @@ __device__ __forceinline__ void ldmatrix_b8_x2_trans(uint32_t (&r)[4], uint32_t 
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
 
+// Block-scaled cache: the accumulators are in units of v_ref / V_BOOST, v_ref a power of two that the warp raises to the
+// largest V scale it has met in the segment (rescaling is exact).  A token's weight is p * rel, rel = vs * V_BOOST / v_ref.
+// p is in [0, 1], and as long as rel is in [V_LEAST, 2 V_BOOST) the fp16 operand p * rel neither overflows nor loses bits to
+// fp16's subnormals for any p >= 2^-19.  A unit with a scale below that range (one block's V 2^8 times smaller than
+// another's in the same segment) is done in passes instead, one per range of scales: a pass has its own reference and
+// its product joins the accumulators in fp32, so that an outlier in one block takes no bits from the others.  Where
+// that is every unit (scales spread over 2^18 at random) 128 x 4096 tokens take 167 us instead of 163.5, 64 x 2048 in pages of 5,
+// with a scale per token, 132 instead of 112.
+constexpr float V_BOOST = 8192.f, V_LEAST = 32.f;
+constexpr float V_REF_MIN = 0x1p-64f, V_REF_MAX = 0x1p126f;   // outputs are fp16: smaller scales are invisible
+__device__ __forceinline__ float power_of_two_below(float x) {   // x positive and normal
+    return __uint_as_float(__float_as_uint(x) & 0x7f800000u);
+}
+
 // grp_row: first token of the group inside the tile; grp_valid (1..32+): how many of its tokens exist.
 //
-// BS: scale_of(t) gives token t's (K scale, V scale) and `qk_scale` is without a K scale.  The V scale joins the softmax
-// as an exponent: y = x + log2(vs) takes x's place in the running maximum and the weights w = 2^(y - m), which
-// therefore stay in [0, 1] with the largest at 1 whatever the scales are (w is rounded to fp16 for the PV
-// product; a plain p * vs would lose bits to fp16's subnormals), and the denominator takes w / vs back out in fp32:
-//   out = sum_t w_t V_t / sum_t w_t / vs_t.   m + log2(sum) is still the log-sum-exp of x, so split rows merge as ever.
+// BS: `qk_scale` is without a K scale.  scale_of(t0, first, lo, hi, live, ks, vs): K and V scales of tokens lo and hi of the 16
+// that start at token t0 of the tile (`first` of the group); a token at or behind `live` does not exist and gets (1, v_ref).
+// v_ref: see above; 0 at a segment's start, where the first block sets it.
 template<bool BS, typename Rows, typename Scales>
 __device__ __forceinline__ bool process_group_e4m3(const uint32_t k_tile, const uint32_t v_tile, const Rows rows,
                                                    const int grp_row, const int grp_valid, const uint32_t (&qb)[8][2],
                                                    float (&acc)[8][4], float (&m_run)[2], float (&l_run)[2],
-                                                   const float qk_scale, const int lane, const Scales scale_of)
+                                                   const float qk_scale, const int lane, const Scales scale_of,
+                                                   float& v_ref)
 {
     const int g = lane >> 2, qd = lane & 3;
     bool wrote = false;
@@ -472,7 +485,7 @@ __device__ __forceinline__ bool process_group_e4m3(const uint32_t k_tile, const 
     // ---- 1. S^T = K Q^T for both 16-token halves, two interleaved accumulators each.
     const int tok_lo = g, tok_hi = tau16(g + 8);      // tokens of MMA rows g, g + 8 within a half
     float x[2][4];
-    float inv_vs[2][2] = {{1.f, 1.f}, {1.f, 1.f}};    // BS: per half and token (lo, hi)
+    float vs[2][2];                                   // BS: per half and token (lo, hi)
 #pragma unroll
     for (int hh = 0; hh < 2; hh++) {
         const uint32_t r0 = rows(grp_row + 16 * hh + tok_lo, 0), r1 = rows(grp_row + 16 * hh + tok_hi, 0);
@@ -491,10 +504,15 @@ __device__ __forceinline__ bool process_group_e4m3(const uint32_t k_tile, const 
             }
         }
         if constexpr (BS) {
-            float ks[2], log_vs[2];
-            scale_of(grp_row + 16 * hh, 16 * hh, tok_lo, tok_hi, grp_valid, ks, log_vs, inv_vs[hh]);
+            float ks[2];
+            if (hh == 0 && v_ref == 0.f) {            // warp-uniform
+                float first[2];
+                scale_of(grp_row, 0, 0, 0, grp_valid, ks, first);
+                v_ref = power_of_two_below(fminf(fmaxf(first[0], V_REF_MIN), V_REF_MAX));
+            }
+            scale_of(grp_row + 16 * hh, 16 * hh, tok_lo, tok_hi, grp_valid, ks, vs[hh]);
 #pragma unroll
-            for (int i = 0; i < 4; i++) x[hh][i] = fmaf(s0[i] + s1[i], qk_scale * ks[i >> 1], log_vs[i >> 1]);
+            for (int i = 0; i < 4; i++) x[hh][i] = (s0[i] + s1[i]) * (qk_scale * ks[i >> 1]);
         } else {
 #pragma unroll
             for (int i = 0; i < 4; i++) x[hh][i] = (s0[i] + s1[i]) * qk_scale;
@@ -525,19 +543,8 @@ __device__ __forceinline__ bool process_group_e4m3(const uint32_t k_tile, const 
     for (int hh = 0; hh < 2; hh++)
 #pragma unroll
         for (int i = 0; i < 4; i++) pr[hh][i] = exp2f(x[hh][i] - m_run[i & 1]);
-    if constexpr (BS) {
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            float sum = pr[0][h] * inv_vs[0][0];
-            sum = fmaf(pr[0][2 + h], inv_vs[0][1], sum);
-            sum = fmaf(pr[1][h], inv_vs[1][0], sum);
-            sum = fmaf(pr[1][2 + h], inv_vs[1][1], sum);
-            l_run[h] = l_run[h] * alpha[h] + sum;
-        }
-    } else {
-        l_run[0] = l_run[0] * alpha[0] + ((pr[0][0] + pr[0][2]) + (pr[1][0] + pr[1][2]));
-        l_run[1] = l_run[1] * alpha[1] + ((pr[0][1] + pr[0][3]) + (pr[1][1] + pr[1][3]));
-    }
+    l_run[0] = l_run[0] * alpha[0] + ((pr[0][0] + pr[0][2]) + (pr[1][0] + pr[1][2]));
+    l_run[1] = l_run[1] * alpha[1] + ((pr[0][1] + pr[0][3]) + (pr[1][1] + pr[1][3]));
     // the accumulators only change scale when some maximum moved, which after the first tiles is rare
     if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
 #pragma unroll
@@ -547,6 +554,77 @@ __device__ __forceinline__ bool process_group_e4m3(const uint32_t k_tile, const 
         }
     }
 
+    // matrix row i of a half = MMA row (k index) 2(i >> 2) + (i & 1) + 8(i >> 1 & 1): the widened low half of a
+    // register is then k = 2qd, 2qd+1 (a0 / a1), the high half k = 2qd+8, 2qd+9 (a2 / a3)
+    const int v_lane = lane & 15;
+    const uint32_t v_row = rows(grp_row + 16 * (lane >> 4) + tau16(2 * (v_lane >> 2) + (v_lane & 1) + 8 * ((v_lane >> 1) & 1)), 0);
+
+    if constexpr (BS) {
+        float rel[2][2];
+        auto weigh = [&](auto outside) {              // rel of the lane's four tokens; does some token of the unit lie outside?
+            const float unit = __uint_as_float(__float_as_uint(V_BOOST) + __float_as_uint(1.f) - __float_as_uint(v_ref));   // V_BOOST / v_ref
+            bool out = false;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                rel[i >> 1][i & 1] = vs[i >> 1][i & 1] * unit;
+                out |= outside(rel[i >> 1][i & 1]);
+            }
+            return __any_sync(0xffffffffu, out);
+        };
+        // (positive floats are ordered like their bits; zeros and NaN lie outside too)
+        if (weigh([](float r) { return __float_as_uint(r) - __float_as_uint(V_LEAST) >= __float_as_uint(2.f * V_BOOST) - __float_as_uint(V_LEAST); })) {
+            auto largest = [&](const float (&s)[2][2]) {
+                float top = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                return top;
+            };
+            const float top = power_of_two_below(fminf(fmaxf(largest(vs), v_ref), V_REF_MAX));
+            const float down = v_ref / top;
+#pragma unroll
+            for (int mt = 0; mt < 8; mt++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) acc[mt][i] *= down;
+            v_ref = top;
+            if (weigh([](float r) { return r < V_LEAST && r != 0.f; })) {      // (a block nothing was ever written to weighs 0)
+                // Tokens of one range of scales after the other, from the largest down: each pass takes at least the block with
+                // the largest scale left.
+                for (;;) {
+                    const float most = largest(vs);
+                    if (!(most > V_REF_MIN)) break;                            // warp-uniform, like the rest of the loop
+                    const float two = power_of_two_below(fminf(most, V_REF_MAX)), back = two / v_ref;
+                    const float unit = __uint_as_float(__float_as_uint(V_BOOST) + __float_as_uint(1.f) - __float_as_uint(two));
+                    uint32_t b[2][2];
+#pragma unroll
+                    for (int hh = 0; hh < 2; hh++)
+#pragma unroll
+                        for (int i = 0; i < 2; i++) {
+                            float w = vs[hh][i] * unit;
+                            if (w >= V_LEAST) vs[hh][i] = 0.f; else w = 0.f;
+                            b[hh][i] = movmatrix_trans(pack_half2(pr[hh][2 * i] * w, pr[hh][2 * i + 1] * w));
+                        }
+#pragma unroll
+                    for (int mt = 0; mt < 8; mt++) {
+                        uint32_t v[4];
+                        ldmatrix_b8_x2_trans(v, v_tile + swz(v_row, mt));
+                        const uint32_t a0[4] = {widen_lo(v[0]), widen_lo(v[1]), widen_hi(v[0]), widen_hi(v[1])};
+                        const uint32_t a1[4] = {widen_lo(v[2]), widen_lo(v[3]), widen_hi(v[2]), widen_hi(v[3])};
+                        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                        mma_16816(sum, a0, b[0][0], b[0][1]);
+                        mma_16816(sum, a1, b[1][0], b[1][1]);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) acc[mt][i] = fmaf(sum[i], back, acc[mt][i]);
+                    }
+                }
+                return wrote;
+            }
+        }
+#pragma unroll
+        for (int hh = 0; hh < 2; hh++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) pr[hh][i] *= rel[hh][i >> 1];
+    }
+
     // ---- 3. O^T += V^T P^T.  P^T's B fragments = transposed 8x8 blocks of the weights (MMA rows 0..7, 8..15).
     uint32_t pb[2][2];
 #pragma unroll
@@ -554,21 +632,14 @@ __device__ __forceinline__ bool process_group_e4m3(const uint32_t k_tile, const 
         pb[hh][0] = movmatrix_trans(pack_half2(pr[hh][0], pr[hh][1]));
         pb[hh][1] = movmatrix_trans(pack_half2(pr[hh][2], pr[hh][3]));
     }
-    {
-        // matrix row i of a half = MMA row (k index) 2(i >> 2) + (i & 1) + 8(i >> 1 & 1): the widened low half of a
-        // register is then k = 2qd, 2qd+1 (a0 / a1), the high half k = 2qd+8, 2qd+9 (a2 / a3)
-        const int i = lane & 15;
-        const int t = grp_row + 16 * (lane >> 4) + tau16(2 * (i >> 2) + (i & 1) + 8 * ((i >> 1) & 1));
-        const uint32_t r = rows(t, 0);
 #pragma unroll
-        for (int mt = 0; mt < 8; mt++) {
-            uint32_t v[4];
-            ldmatrix_b8_x2_trans(v, v_tile + swz(r, mt));
-            const uint32_t a0[4] = {widen_lo(v[0]), widen_lo(v[1]), widen_hi(v[0]), widen_hi(v[1])};
-            const uint32_t a1[4] = {widen_lo(v[2]), widen_lo(v[3]), widen_hi(v[2]), widen_hi(v[3])};
-            mma_16816(acc[mt], a0, pb[0][0], pb[0][1]);
-            mma_16816(acc[mt], a1, pb[1][0], pb[1][1]);
-        }
+    for (int mt = 0; mt < 8; mt++) {
+        uint32_t v[4];
+        ldmatrix_b8_x2_trans(v, v_tile + swz(v_row, mt));
+        const uint32_t a0[4] = {widen_lo(v[0]), widen_lo(v[1]), widen_hi(v[0]), widen_hi(v[1])};
+        const uint32_t a1[4] = {widen_lo(v[2]), widen_lo(v[3]), widen_hi(v[2]), widen_hi(v[3])};
+        mma_16816(acc[mt], a0, pb[0][0], pb[0][1]);
+        mma_16816(acc[mt], a1, pb[1][0], pb[1][1]);
     }
     return wrote;
 }
@@ -890,6 +961,7 @@ paged_decode_kernel(const __grid_constant__ pd_params p, const __grid_constant__
     // softmax runs in base 2; with per-head scales the factor belongs to the segment's kv head
     float qk_scale = p.sm_scale * p.k_scale * 1.4426950408889634f;
     float v_scale  = p.v_scale;
+    float v_ref = 0.f;          // block-scaled: unit of the accumulators, see V_BOOST; v_scale is then 1 until a segment's end
     if constexpr (BS) { qk_scale = p.sm_scale * 1.4426950408889634f; v_scale = 1.f; }
     if constexpr (S::HEADS > 1 && !BS) {
         if (hs.k) qk_scale = p.sm_scale * __ldg(hs.k + warp) * 1.4426950408889634f;
@@ -947,6 +1019,7 @@ paged_decode_kernel(const __grid_constant__ pd_params p, const __grid_constant__
         for (int mt = 0; mt < 8; mt++) acc[mt][0] = acc[mt][1] = acc[mt][2] = acc[mt][3] = 0.f;
         m_run[0] = m_run[1] = -INFINITY;
         l_run[0] = l_run[1] = 0.f;
+        v_ref = 0.f;
 
         for (int tok = sg.z; tok < sg.w; tok += S::TILE) {
             const int stage = c_stage;
@@ -988,26 +1061,23 @@ paged_decode_kernel(const __grid_constant__ pd_params p, const __grid_constant__
                 const int box_head = S::HEADS > 1 ? warp : 0;
                 auto rows = [&](int t, int panel) { return row_offset<KV, S::HEADS>(t, panel, btl, box_head); };
                 if constexpr (FP8) {
-                    // (K scale, log2 and reciprocal of the V scale) of the lane's two tokens of a 16-token half; tokens that
-                    // do not exist, and blocks nothing was ever written to (zeros), count as scale 1
+                    // K and V scales of the lane's two tokens of a 16-token half
                     const uint32_t slot = pipe + S::SCALE_OFFSET + stage * S::scale_slot_bytes(bs.log2_block);
-                    auto scale_of = [&](int t0, int first, int lo, int hi, int live, float (&ks)[2], float (&log_vs)[2], float (&inv)[2]) {
+                    auto scale_of = [&](int t0, int first, int lo, int hi, int live, float (&ks)[2], float (&vs)[2]) {
 #pragma unroll
                         for (int i = 0; i < 2; i++) {
-                            if (i == 1 && bs.log2_block == 4) { ks[1] = ks[0]; log_vs[1] = log_vs[0]; inv[1] = inv[0]; break; }
+                            if (i == 1 && bs.log2_block == 4) { ks[1] = ks[0]; vs[1] = vs[0]; break; }
                             const int in_half = bs.log2_block == 4 ? 0 : i ? hi : lo;
-                            float2 kv = make_float2(1.f, 1.f);
+                            float2 kv = make_float2(1.f, v_ref);
                             if (first + in_half < live) {
                                 const uint2 raw = lds64(slot + (((t0 + in_half) >> bs.log2_block) * S::HEADS + box_head) * 8);
                                 kv = make_float2(__uint_as_float(raw.x), __uint_as_float(raw.y));
-                                if (!(kv.y > 0.f)) kv.y = 1.f;
                             }
                             ks[i] = kv.x;
-                            log_vs[i] = __log2f(kv.y);
-                            inv[i] = __fdividef(1.f, kv.y);
+                            vs[i] = kv.y;
                         }
                     };
-                    wrote |= process_group_e4m3<BS>(k_tile, v_tile, rows, grp_row, grp_valid, qb, acc, m_run, l_run, qk_scale, lane, scale_of);
+                    wrote |= process_group_e4m3<BS>(k_tile, v_tile, rows, grp_row, grp_valid, qb, acc, m_run, l_run, qk_scale, lane, scale_of, v_ref);
                 }
                 else
                     wrote |= process_group_f16(k_tile, v_tile, rows, grp_row, grp_valid, qb, acc, m_run, l_run, qk_scale, lane);
@@ -1026,6 +1096,13 @@ paged_decode_kernel(const __grid_constant__ pd_params p, const __grid_constant__
         // Accumulator mt of a lane: dims 16mt + g (values 0, 1) and 16mt + g + 8 (values 2, 3), heads 2qd, 2qd+1.
         {
             float l[2] = {l_run[0], l_run[1]};
+            if constexpr (BS) {
+                const float unit = v_ref / V_BOOST;
+#pragma unroll
+                for (int mt = 0; mt < 8; mt++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) acc[mt][i] *= unit;
+            }
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) {
                 l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
