@@ -53,6 +53,13 @@ int set_error(int code, const char* fmt, ...) {
                              __FILE__, __LINE__, cudaGetErrorString(e_));                  \
     } while (0)
 
+// New device memory, zeroed when this returns.  cudaMemset alone only queues the zeros, on the legacy default stream behind
+// whatever is there; a non-blocking stream that uses the memory next would not wait for them.
+cudaError_t zeroed_now(void* p, size_t bytes) {
+    const cudaError_t e = cudaMemset(p, 0, bytes);
+    return e == cudaSuccess ? cudaStreamSynchronize(cudaStreamLegacy) : e;
+}
+
 // ---- kernel shapes --------------------------------------------------------------------
 // CTA shape and pipeline depth per cache dtype: Config<consumer warps, 16-token groups per warp per tile,
 // stages, CTAs per SM>, plus one producer warp per CTA.  fp16: 4 warps, 64-token tiles, 3 stages of 32 KB, two
@@ -2034,7 +2041,7 @@ int pd_cache_set_block_scales(pd_cache* c, int on) {
     const size_t pairs = static_cast<size_t>(c->cfg.num_pages) * c->cfg.num_kv_heads * (c->cfg.page_size >> scale_block_log2(c->cfg.page_size));
     float* scales = nullptr;
     PD_CUDA(cudaMalloc(&scales, 2 * sizeof(float) * pairs));
-    const cudaError_t e = cudaMemset(scales, 0, 2 * sizeof(float) * pairs);   // 0: nothing written yet
+    const cudaError_t e = zeroed_now(scales, 2 * sizeof(float) * pairs);   // 0: nothing written yet
     if (e != cudaSuccess) { cudaFree(scales); return set_error(PD_CUDA_ERROR, "set_block_scales: %s", cudaGetErrorString(e)); }
     c->d_block_scales = scales;
     return PD_OK;
