@@ -56,8 +56,8 @@ RateTable* rate_table(const void* fn, int grid, bool create = true) {
         void* dev_mem = nullptr;
         void* host = nullptr;
         void* share_mem = nullptr;
-        if (cudaMalloc(&dev_mem, bytes) != cudaSuccess || cudaMemset(dev_mem, 0, bytes) != cudaSuccess ||
-            cudaMalloc(&share_mem, share_bytes) != cudaSuccess || cudaMemset(share_mem, 0, share_bytes) != cudaSuccess ||
+        if (cudaMalloc(&dev_mem, bytes) != cudaSuccess || zeroed_now(dev_mem, bytes) != cudaSuccess ||
+            cudaMalloc(&share_mem, share_bytes) != cudaSuccess || zeroed_now(share_mem, share_bytes) != cudaSuccess ||
             cudaMallocHost(&host, bytes) != cudaSuccess ||
             cudaEventCreateWithFlags(&t.copied, cudaEventDisableTiming) != cudaSuccess) {
             cudaGetLastError();

@@ -247,7 +247,7 @@ int status_word(unsigned** out) {
     std::lock_guard<std::mutex> lock(g_status_mutex);
     if (!g_status[dev]) {
         PD_CUDA(cudaMalloc(&g_status[dev], sizeof(unsigned)));
-        PD_CUDA(cudaMemset(g_status[dev], 0, sizeof(unsigned)));
+        PD_CUDA(zeroed_now(g_status[dev], sizeof(unsigned)));
     }
     *out = g_status[dev];
     return PD_OK;
@@ -1320,7 +1320,7 @@ int pd_kernel_status(void* stream, unsigned* out) {
     PD_CUDA(cudaStreamSynchronize(static_cast<cudaStream_t>(stream)));
     PD_CUDA(cudaMemcpy(out, status, sizeof(unsigned), cudaMemcpyDeviceToHost));
     if (*out) {
-        PD_CUDA(cudaMemset(status, 0, sizeof(unsigned)));
+        PD_CUDA(zeroed_now(status, sizeof(unsigned)));
         if ((*out >> 24) == pdk::ST_WORKSPACE)
             return set_error(PD_KERNEL_TIMEOUT, "decode kernel: the plan has more segments than the workspace holds (CTA %u gave up)",
                              *out & 0xffffffu);
@@ -1415,7 +1415,7 @@ int pd_gather_create(int world, int rank, size_t out_bytes, pd_gather_group** ou
     g->block_bytes = GATHER_BUFFERS * g->out_bytes + 256;
     void* b = nullptr;
     cudaError_t e = cudaMalloc(&b, g->block_bytes);
-    if (e == cudaSuccess) e = cudaMemset(b, 0, g->block_bytes);
+    if (e == cudaSuccess) e = zeroed_now(b, g->block_bytes);
     if (e != cudaSuccess) {
         cudaFree(b);
         delete g;
@@ -1603,11 +1603,11 @@ int pd_cache_create(const pd_cache_config* cfg, pd_cache** out) {
     // Pools start as zeros: the decode kernel copies whole pages, and bytes a sequence
     // never wrote must not decode to NaN.
     PD_CACHE_CUDA(cudaMemset(c->d_k, 0, half_bytes));
-    PD_CACHE_CUDA(cudaMemset(c->d_v, 0, half_bytes));
+    PD_CACHE_CUDA(cudaMemset(c->d_v, 0, half_bytes));      // (waited for below, with the lengths)
     PD_CACHE_CUDA(cudaMalloc(&c->d_block_table, table_bytes));
     PD_CACHE_CUDA(cudaMalloc(&c->d_seq_lens, sizeof(int) * cfg->max_slots));
     PD_CACHE_CUDA(cudaMemset(c->d_block_table, 0, table_bytes));
-    PD_CACHE_CUDA(cudaMemset(c->d_seq_lens, 0, sizeof(int) * cfg->max_slots));
+    PD_CACHE_CUDA(zeroed_now(c->d_seq_lens, sizeof(int) * cfg->max_slots));
 #undef PD_CACHE_CUDA
     if (int rc = pd_device_plan_create(&c->device_plan)) return fail(rc);
     // Pages are taken from the back of the list; page 0 goes out first.

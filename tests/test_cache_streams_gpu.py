@@ -35,3 +35,32 @@ def test_block_scales_are_zeroed_before_the_first_append(torch_cuda, pa):
     torch.cuda.synchronize()
     s = block_scales(c, torch)
     assert (s[c.block_table(slot)[0]] == 2.0 ** -8).all() and (s == 0).sum() == s.numel() - 4
+
+
+def test_a_new_cache_is_zeroed_before_the_first_append(torch_cuda, pa):
+    """Pools, block table and lengths; the device-side plan reads the last two."""
+    torch = torch_cuda
+    hkv, hq = 2, 4
+    side = torch.cuda.Stream()
+    g = torch.Generator(device="cuda").manual_seed(1)
+    k, v = (torch.randn(40, hkv, 128, device="cuda", generator=g).half() for _ in range(2))
+    q = torch.randn(1, hq, 128, device="cuda", generator=g).half()
+    out = torch.zeros_like(q)
+    rows = pa.qkv_params(None, k, v)
+    pa.kernel_status()
+    torch.cuda.synchronize()
+    torch.cuda._sleep(QUEUED)
+    c = new_cache(pa, dtype=0)
+    slots = [c.admit() for _ in range(2)]
+    assert c.append_qkv(slots[1:], [40], rows, None, None, side.cuda_stream)
+    torch.cuda.synchronize()
+    assert device_view(c.params().seq_lens, 16, torch).view(torch.int32).tolist() == [0, 40, 0, 0]
+    pool = device_view(c.params().k_cache, 8 * hkv * 16 * 128 * 2, torch).view(torch.float16).view(8, hkv, 16, 128)
+    pages = c.block_table(1)
+    assert torch.equal(pool[torch.from_numpy(pages[:2].astype(np.int64)).cuda()].transpose(1, 2).reshape(32, hkv, 128), k[:32])
+    assert not pool[int(pages[2]), :, 8:].any()
+    c.plan([1], hq)
+    c.run(q, out)
+    assert pa.kernel_status() == 0
+    want, tol = ro.attention(q[0].double().cpu().numpy(), k.double().cpu().numpy(), v.double().cpu().numpy(), 1 / np.sqrt(np.float32(128)))
+    assert (np.abs(out[0].double().cpu().numpy() - want) <= tol).all()
