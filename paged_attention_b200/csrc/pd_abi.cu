@@ -404,6 +404,8 @@ struct pd_cache {
     void*  batch_staging = nullptr;
     void*  batch_device = nullptr;
     size_t batch_cap = 0;
+    cudaEvent_t released = nullptr;       // behind the latest release's zero of a slot's device length
+    bool   release_pending = false;
     cudaEvent_t batch_staged = nullptr;
     cudaEvent_t batch_done = nullptr;     // the last batched append's kernels (release waits for them)
     bool batch_pending = false;
@@ -1567,6 +1569,7 @@ void pd_cache_destroy(pd_cache* c) {
     cudaFree(c->d_slot_ids);
     cudaFree(c->d_head_scales);
     cudaFree(c->d_block_scales);
+    if (c->released) cudaEventDestroy(c->released);
     if (c->batch_staged) { cudaEventSynchronize(c->batch_staged); cudaEventDestroy(c->batch_staged); }
     if (c->batch_done) { cudaEventSynchronize(c->batch_done); cudaEventDestroy(c->batch_done); }
     cudaFreeHost(c->batch_staging);
@@ -1629,6 +1632,15 @@ int pd_cache_admit(pd_cache* c) {
 
 }  // extern "C"
 namespace {
+// release() queues its zero of the slot's device length on the default stream, behind the kernels there that may still read the
+// old one; what writes or reads the lengths next waits for it on its own stream.
+int wait_for_release(pd_cache* c, cudaStream_t stream) {
+    if (!c->release_pending) return PD_OK;
+    PD_CUDA(cudaStreamWaitEvent(stream, c->released, 0));
+    if (cudaEventQuery(c->released) == cudaSuccess) c->release_pending = false;
+    else cudaGetLastError();
+    return PD_OK;
+}
 // The cache as the target of an append; the caller adds which sequences.
 int cache_pages(pd_cache* c, pdk::PageArgs* t) {
     *t = pdk::PageArgs{};
@@ -1683,6 +1695,7 @@ int pd_cache_append(pd_cache* c, int slot, const void* d_k, const void* d_v, int
         c->free_pages.pop_back();
     }
     int* row = c->d_block_table + static_cast<size_t>(slot) * c->cfg.max_pages_per_slot;
+    if (int rc = wait_for_release(c, stream)) return rc;
     // Pageable-source copies are staged by the driver before they return.
     if (need > have)
         PD_CUDA(cudaMemcpyAsync(row + have, c->tables[slot].data() + have, sizeof(int) * (need - have),
@@ -1814,6 +1827,7 @@ int append_batch_impl(pd_cache* c, int count, const int* slots, const void* cons
     if (as_rows) begin[count] = token;
     // the previous batch's kernels, perhaps on another stream, still read the device copy of their lists
     if (c->batch_pending) PD_CUDA(cudaStreamWaitEvent(stream, c->batch_done, 0));
+    if (int rc = wait_for_release(c, stream)) return rc;
     PD_CUDA(cudaMemcpyAsync(c->batch_device, c->batch_staging, total, cudaMemcpyHostToDevice, stream));
     PD_CUDA(cudaEventRecord(c->batch_staged, stream));
     char* d = static_cast<char*>(c->batch_device);
@@ -1899,6 +1913,9 @@ int pd_cache_release(pd_cache* c, int slot) {
     c->seq_lens[slot] = 0;
     c->occupied[slot] = 0;
     PD_CUDA(cudaMemset(c->d_seq_lens + slot, 0, sizeof(int)));
+    if (!c->released) PD_CUDA(cudaEventCreateWithFlags(&c->released, cudaEventDisableTiming));
+    PD_CUDA(cudaEventRecord(c->released, cudaStreamLegacy));
+    c->release_pending = true;
     return PD_OK;
 }
 
@@ -1964,6 +1981,11 @@ int pd_cache_plan_device(pd_cache* c, const int* d_slot_ids, int batch, int num_
     if (!c) return set_error(PD_INVALID_ARGUMENT, "plan_device: null cache");
     if (batch < 0 || (!d_slot_ids && batch > c->cfg.max_slots))
         return set_error(PD_INVALID_ARGUMENT, "plan_device: batch exceeds the cache's slots");
+    // (a capture cannot wait for what was queued before it; its replays come after)
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    if (c->release_pending && cudaStreamIsCapturing(static_cast<cudaStream_t>(stream), &capture) == cudaSuccess &&
+        capture == cudaStreamCaptureStatusNone)
+        if (int rc = wait_for_release(c, static_cast<cudaStream_t>(stream))) return rc;
     if (int rc = pd_device_plan_build(c->device_plan, c->cfg.dtype, c->d_seq_lens, d_slot_ids, batch, num_q_heads,
                                       c->cfg.num_kv_heads, c->cfg.head_dim, num_ctas, stream))
         return rc;

@@ -64,3 +64,49 @@ def test_a_new_cache_is_zeroed_before_the_first_append(torch_cuda, pa):
     assert pa.kernel_status() == 0
     want, tol = ro.attention(q[0].double().cpu().numpy(), k.double().cpu().numpy(), v.double().cpu().numpy(), 1 / np.sqrt(np.float32(128)))
     assert (np.abs(out[0].double().cpu().numpy() - want) <= tol).all()
+
+
+@pytest.mark.parametrize("batched", [False, True])
+def test_a_released_slot_is_zeroed_before_its_next_append(batched, torch_cuda, pa):
+    """release() zeroes the slot's device length, which the device-side plan reads, on the default stream."""
+    torch = torch_cuda
+    hkv, hq = 2, 4
+    side = torch.cuda.Stream()
+    g = torch.Generator(device="cuda").manual_seed(2)
+    k, v = (torch.randn(40, hkv, 128, device="cuda", generator=g).half() for _ in range(2))
+    q = torch.randn(1, hq, 128, device="cuda", generator=g).half()
+    out = torch.zeros_like(q)
+    c = new_cache(pa, dtype=0)
+    assert c.admit() == 0 and c.append(0, v, k, 17)
+    torch.cuda.synchronize()
+    torch.cuda._sleep(QUEUED)
+    c.release(0)
+    assert c.admit() == 0
+    if batched:
+        assert c.append_batch([0], [k], [v], [40], side.cuda_stream)
+    else:
+        assert c.append(0, k, v, 40, side.cuda_stream)
+    c.plan_device(1, hq, stream=side.cuda_stream)
+    c.run(q, out, side.cuda_stream)
+    torch.cuda.synchronize()
+    assert pa.kernel_status() == 0
+    assert device_view(c.params().seq_lens, 16, torch).view(torch.int32).tolist() == [40, 0, 0, 0]
+    want, tol = ro.attention(q[0].double().cpu().numpy(), k.double().cpu().numpy(), v.double().cpu().numpy(), 1 / np.sqrt(np.float32(128)))
+    assert (np.abs(out[0].double().cpu().numpy() - want) <= tol).all()
+
+
+def test_a_device_plan_sees_a_released_slot_as_empty(torch_cuda, pa):
+    torch = torch_cuda
+    side = torch.cuda.Stream()
+    x = torch.ones(40, 2, 128, dtype=torch.float16, device="cuda")
+    q, out = torch.ones(2, 4, 128, dtype=torch.float16, device="cuda"), torch.full((2, 4, 128), 7.0, dtype=torch.float16, device="cuda")
+    c = new_cache(pa, dtype=0)
+    assert [c.admit(), c.admit()] == [0, 1] and c.append(0, x, x, 40) and c.append(1, x, x, 20)
+    torch.cuda.synchronize()
+    torch.cuda._sleep(QUEUED)
+    c.release(0)
+    c.plan_device(2, 4, stream=side.cuda_stream)
+    c.run(q, out, side.cuda_stream)
+    torch.cuda.synchronize()
+    assert pa.kernel_status() == 0
+    assert (out[0] == 7).all() and (out[1] == 1).all()          # a row of length 0 is left as it was
