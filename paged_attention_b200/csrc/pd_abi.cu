@@ -1695,6 +1695,9 @@ int pd_cache_append(pd_cache* c, int slot, const void* d_k, const void* d_v, int
         c->free_pages.pop_back();
     }
     int* row = c->d_block_table + static_cast<size_t>(slot) * c->cfg.max_pages_per_slot;
+    // A batched append, perhaps on another stream, still writes this slot's table entries and length, and (block scales) the
+    // begun block that these tokens join.
+    if (c->batch_pending) PD_CUDA(cudaStreamWaitEvent(stream, c->batch_done, 0));
     if (int rc = wait_for_release(c, stream)) return rc;
     // Pageable-source copies are staged by the driver before they return.
     if (need > have)
@@ -1719,6 +1722,7 @@ int pd_cache_append(pd_cache* c, int slot, const void* d_k, const void* d_v, int
         return rc;
     // As in the reference (src/decode/paged_kv_cache.cu:133-134) the call returns with the tokens in place.
     PD_CUDA(cudaStreamSynchronize(stream));
+    c->batch_pending = false;              // waited for above
     return PD_OK;
 }
 

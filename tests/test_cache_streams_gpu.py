@@ -110,3 +110,48 @@ def test_a_device_plan_sees_a_released_slot_as_empty(torch_cuda, pa):
     torch.cuda.synchronize()
     assert pa.kernel_status() == 0
     assert (out[0] == 7).all() and (out[1] == 1).all()          # a row of length 0 is left as it was
+
+
+@pytest.mark.parametrize("blocks", [False, True])
+def test_single_and_batched_appends_on_two_streams(blocks, torch_cuda, pa):
+    """append_qkv and append_batch on one stream, kept busy, and append on another, for the same slots: lengths, tables, bytes and
+    scales as from the same calls with waits in between."""
+    torch = torch_cuda
+    hkv, pages = 2, 24
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    rng = np.random.default_rng(3)
+    # magnitudes that grow: with block scales every call re-encodes what the one before it left in the block
+    x = torch.from_numpy(rng.standard_normal((12, 2, 5, hkv, 128)) * 2.0 ** np.arange(12)[:, None, None, None, None]).half().cuda()
+    results = []
+    for wait in (True, False):
+        c = new_cache(pa, pages=pages, slots=2, per_slot=12)
+        if blocks:
+            c.set_block_scales()
+        slots = [c.admit(), c.admit()]
+        torch.cuda.synchronize()
+
+        def then():
+            if wait:
+                torch.cuda.synchronize()
+        for i in range(12):
+            rows = x[i].reshape(10, hkv, 128)
+            if not wait:
+                with torch.cuda.stream(a):
+                    torch.cuda._sleep(QUEUED // 20)
+            if i % 3:
+                assert c.append_qkv(slots, [5, 5], pa.qkv_params(None, rows, rows), None, None, a.cuda_stream)
+            else:
+                assert c.append_batch(slots, [x[i, 0], x[i, 1]], [x[i, 1], x[i, 0]], [5, 4], a.cuda_stream)
+            then()
+            assert c.append(slots[i % 2], x[i, 0], x[i, 1], 3, b.cuda_stream)
+            then()
+        torch.cuda.synchronize()
+        assert pa.kernel_status() == 0
+        p, bytes_ = c.params(), pages * hkv * 16 * 128
+        state = [device_view(ptr, n, torch).clone() for ptr, n in ((p.k_cache, bytes_), (p.v_cache, bytes_), (p.seq_lens, 8), (p.block_table, 2 * 12 * 4))]
+        if blocks:
+            state.append(device_view(c.block_scales(), pages * hkv * 8, torch).clone())
+        results.append(state)
+        assert state[2].view(torch.int32).tolist() == [c.seq_len(s) for s in slots] == [78, 74]
+        c.close()
+    assert all(torch.equal(s, t) for s, t in zip(*results))
