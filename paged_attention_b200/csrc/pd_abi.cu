@@ -1682,6 +1682,7 @@ int pd_cache_append(pd_cache* c, int slot, const void* d_k, const void* d_v, int
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     const int ps = c->cfg.page_size;
     const int old_len = c->seq_lens[slot];
+    if (n > 0x7fffffff - old_len - ps) return set_error(PD_LENGTH_ERROR, "append: sequence exceeds max_pages_per_slot");
     const int new_len = old_len + n;
     const int have = static_cast<int>(c->tables[slot].size());
     const int need = (new_len + ps - 1) / ps;

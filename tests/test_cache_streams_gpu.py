@@ -1,5 +1,5 @@
 """Calls on a cache from streams that do not wait for each other (every torch side stream is a non-blocking one), with work
-still queued on the stream that a call uses inside."""
+still queued on the stream that a call uses inside; lengths that do not fit."""
 import numpy as np
 import pytest
 
@@ -155,3 +155,21 @@ def test_single_and_batched_appends_on_two_streams(blocks, torch_cuda, pa):
         assert state[2].view(torch.int32).tolist() == [c.seq_len(s) for s in slots] == [78, 74]
         c.close()
     assert all(torch.equal(s, t) for s, t in zip(*results))
+
+
+@pytest.mark.parametrize("dtype, blocks", [(0, False), (1, False), (1, True)])
+def test_a_length_past_31_bits_is_refused(dtype, blocks, torch_cuda, pa):
+    """Nothing may be launched for it: a sum that wraps would pass the check against max_pages_per_slot."""
+    torch = torch_cuda
+    x = torch.ones(3, 2, 128, dtype=torch.float16, device="cuda")
+    c = new_cache(pa, dtype=dtype)
+    if blocks:
+        c.set_block_scales()
+    slot = c.admit()
+    assert c.append(slot, x, x, 3)
+    for n in (2 ** 31 - 1, 2 ** 31 - 3, 2 ** 31 - 16, 4 * 16 - 2):
+        with pytest.raises(pa.LengthError):
+            c.append(slot, x, x, n)
+        with pytest.raises(pa.LengthError):
+            c.append_batch([slot], [x], [x], [n])
+    assert c.seq_len(slot) == 3 and c.free_pages() == 7
