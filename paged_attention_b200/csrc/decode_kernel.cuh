@@ -822,6 +822,17 @@ paged_decode_kernel(const __grid_constant__ pd_params p, const __grid_constant__
             const int slot = p.slot_ids ? __ldg(p.slot_ids + b) : b;
             return p.block_table + static_cast<size_t>(slot) * p.block_table_stride;
         };
+        // the page of the box that starts at token t (row_gather: of each of its four tokens)
+        auto box_pages = [&](const int* table, int t, int end) {
+            int4 pg = make_int4(__ldg(table + t / ps), 0, 0, 0);
+            if (S::HEADS == 1 && row_gather) {
+                const int last = end - 1;
+                pg.y = __ldg(table + min(t + 1, last) / ps);
+                pg.z = __ldg(table + min(t + 2, last) / ps);
+                pg.w = __ldg(table + min(t + 3, last) / ps);
+            }
+            return pg;
+        };
         // Issue the copies of one tile: lanes [lane0, lane0 + nb) own one box each when
         // the tile has <= 32 boxes, otherwise every lane walks boxes lane, lane+32, ...
         auto issue_tile = [&](const int4& sg, int tile_tok, int4 my_page, int lane0, const int* bt) -> bool {
@@ -874,8 +885,7 @@ paged_decode_kernel(const __grid_constant__ pd_params p, const __grid_constant__
                 const int j = lane - lane0;
                 if (j >= 0 && j < nb) copy_box(j, my_page);
             } else {
-                for (int j = lane; j < nb; j += 32)
-                    copy_box(j, make_int4(__ldg(bt + (tile_tok + (j << btl)) / ps), 0, 0, 0));
+                for (int j = lane; j < nb; j += 32) copy_box(j, box_pages(bt, tile_tok + (j << btl), sg.w));
             }
             if constexpr (BS) {
                 // the tile's scale pairs, one per lane and round; a block never straddles a box
@@ -888,7 +898,8 @@ paged_decode_kernel(const __grid_constant__ pd_params p, const __grid_constant__
                     const int t = e / S::HEADS << bs.log2_block;     // first token of the block, within the tile
                     const int head = S::HEADS == 1 ? sg.y : e % S::HEADS;
                     int pg = __shfl_sync(0xffffffffu, my_page.x, lane0 + (t >> btl));
-                    if (S::HEADS == 1 && row_gather) pg = __ldg(bt + (tile_tok + t) / ps);   // several pages to a box
+                    // several pages to a box, or more boxes than lanes
+                    if ((S::HEADS == 1 && row_gather) || bpt > 32) pg = __ldg(bt + (tile_tok + t) / ps);
                     const bool live = pg >= 0 && pg < bs.num_pages;
                     const float2* src = bs.scales + (static_cast<size_t>(live ? pg : 0) * p.num_kv_heads + head) * per_page
                                         + ((tile_tok + t) % ps >> bs.log2_block);
@@ -908,20 +919,10 @@ paged_decode_kernel(const __grid_constant__ pd_params p, const __grid_constant__
         int4 sg  = __ldg(segments + seg);
         const int* bt = table_of(sg.x);
         int  tok = sg.z;
-        // the page id of this lane's box (row_gather: of each of its four tokens)
+        // the pages of this lane's box of a chunk
         auto page_of = [&](const int4& s, const int* table, int chunk_tok) {
             const int t = chunk_tok + (lane << btl);
-            int4 pg = make_int4(0, 0, 0, 0);
-            if (bpt <= 32 && t < s.w) {
-                pg.x = __ldg(table + t / ps);
-                if (S::HEADS == 1 && row_gather) {
-                    const int last = s.w - 1;
-                    pg.y = __ldg(table + min(t + 1, last) / ps);
-                    pg.z = __ldg(table + min(t + 2, last) / ps);
-                    pg.w = __ldg(table + min(t + 3, last) / ps);
-                }
-            }
-            return pg;
+            return bpt <= 32 && t < s.w ? box_pages(table, t, s.w) : make_int4(0, 0, 0, 0);
         };
         int4 page = page_of(sg, bt, tok);
         while (ok && seg < seg_end) {
