@@ -388,7 +388,8 @@ int pd_scale_block_tokens(int page_size);
  *     code 7 with the row.
  *   - No two sequences of a call may write the same page.
  *   - fp8 cache: per-tensor scales, d_k_scales / d_v_scales per kv head, or d_block_scales.  The stored byte is
- *     e4m3(value / scale), rounded once from fp32 to nearest even and saturating; a NaN stays one.
+ *     e4m3(value * (1 / scale)) with both factors in fp32, the reciprocal correctly rounded (as in pd_append_tokens_scaled:
+ *     rows without norm and rotation leave the same bytes), to nearest even and saturating; a NaN stays one.
  *   - d_block_scales [num_pages][num_kv_heads][page_size / block][2] (K, V): every block that receives tokens gets the
  *     smallest power of two (2^-32 .. 2^8) that brings its largest new magnitude to at most 448; a block that was begun
  *     by an earlier call keeps its scale if that is larger, otherwise the rest of the block is re-encoded (an

@@ -628,7 +628,9 @@ rows_kernel(const __grid_constant__ RowArgs a, const __grid_constant__ RopeArgs 
 #pragma unroll 1
         for (; unit < end; unit += step) {
             float factor = inv;
-            if (quantised && head_scales) factor = __fdividef(1.f, head_scales[min(4 * (unit - first) + sh, a.hkv - 1)]);
+            // times the correctly rounded reciprocal, as the append of plain rows does: both leave the same bytes in a cache (a
+            // division per value would take 13 % longer: 54.2 us for the ragged chunks above)
+            if (quantised && head_scales) factor = __frcp_rn(head_scales[min(4 * (unit - first) + sh, a.hkv - 1)]);
             cp_async_wait<ROWS_SLOTS - 1>();
             Vals x = unpack<ACT>(Raw{load_shared(&slots[warp][slot][0][lane]), load_shared(&slots[warp][slot][1][lane])});
             fetch(unit + ROWS_SLOTS * step, slot);
