@@ -447,8 +447,8 @@ int    pd_cache_release(pd_cache* c, int slot);
 int    pd_cache_set_head_scales(pd_cache* c, const float* k_scales, const float* v_scales);
 /* One scale per (block of tokens, kv head) for K and for V instead of the config's per-tensor scales (fp8 cache; on = 0:
  * back to those).  Every later append quantises with them, as pd_append_qkv does, and every later run reads them.
- * The params of such a cache (pd_cache_params) carry NaN as k_scale and v_scale, which this decode ignores and any
- * decode that does not take the block scales turns into NaN instead of silently wrong numbers.
+ * The params of such a cache (pd_cache_params) carry NaN as k_scale and v_scale, which pd_paged_decode_block_scaled
+ * ignores; every decode that does not take the block scales (plain, static, gathered) refuses them.
  * Only while the cache holds no tokens and without head scales.  Adds 8 bytes per block and kv head, which
  * pd_cache_bytes_per_page and pd_cache_total_bytes do not count.  No counterpart in the reference. */
 int    pd_cache_set_block_scales(pd_cache* c, int on);

@@ -1109,6 +1109,12 @@ Selection select_schedule(int dtype, const pd_params* p, const KernelInfo* k, bo
     return sel;
 }
 
+// The params of a block-scaled cache carry NaN scales; a decode that would use them has not been given the block scales.
+int check_scales(const char* who, int dtype, const pd_params* p, const pdk::HeadScales& heads) {
+    if (dtype != PD_FP8_E4M3 || ((heads.k || !std::isnan(p->k_scale)) && (heads.v || !std::isnan(p->v_scale)))) return PD_OK;
+    return set_error(PD_INVALID_ARGUMENT, "%s: the scales are NaN (a block-scaled cache takes pd_paged_decode_block_scaled)", who);
+}
+
 int decode_impl(int dtype, const pd_params* p, int num_pages, const pdk::GatherOut& gather, void* stream_,
                 const pdk::HeadScales& scales = pdk::HeadScales{nullptr, nullptr},
                 const float* block_scales = nullptr) {
@@ -1118,6 +1124,8 @@ int decode_impl(int dtype, const pd_params* p, int num_pages, const pdk::GatherO
     const KernelInfo* k;
     if (int rc = find_kernel(dtype, p->head_dim, p->num_q_heads / p->num_kv_heads, &k)) return rc;
     if (p->page_size <= 0) return set_error(PD_INVALID_ARGUMENT, "page_size must be positive");
+    if (!block_scales)
+        if (int rc = check_scales("paged_decode", dtype, p, scales)) return rc;
     if (p->num_ctas <= 0 || p->batch <= 0) return PD_OK;   // empty plan: nothing to do
     if (!p->q || (!p->out && !gather.world) || !p->k_cache || !p->v_cache || !p->block_table || !p->segments ||
         !p->cta_seg_begin || !p->item_seg_begin)
@@ -1269,6 +1277,7 @@ int pd_paged_decode_static(int dtype, const pd_params* p, int num_segments, int 
     const KernelInfo* k;
     if (int rc = find_kernel(dtype, p->head_dim, group, &k)) return rc;
     if (p->page_size <= 0) return set_error(PD_INVALID_ARGUMENT, "page_size must be positive");
+    if (int rc = check_scales("paged_decode_static", dtype, p, pdk::HeadScales{nullptr, nullptr})) return rc;
     if (num_segments < 0) return set_error(PD_INVALID_ARGUMENT, "paged_decode_static: num_segments must not be negative");
     const size_t rows = static_cast<size_t>(num_segments) * group;
     const size_t need = rows * (p->head_dim + 1);
