@@ -458,22 +458,12 @@ __device__ __forceinline__ float power_of_two_below(float x) {   // x positive a
     return __uint_as_float(__float_as_uint(x) & 0x7f800000u);
 }
 
-// Block-scaled weights go to the tensor cores as two fp16 terms, so that the result is as exact as with fp32 weights (one term, the
-// choice of the decodes without block scales, rounds a weight by up to 2^-11, like the output).  Groups of up to four
-// query heads (TWINS) leave half of an MMA's eight columns free: columns 4..7 repeat the query rows of columns 0..3, arrive at
-// the same scores and weights, and carry the second term; the two halves are added at a segment's end.  Groups of eight take a
-// second MMA.  Neither shows in the time: 128 x 4096 tokens 162.3 us with one term and with two, 16 x 4096 with groups of eight 30.1.
-__device__ __forceinline__ uint32_t second_term(float a, float b, uint32_t first) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&first));
-    return pack_half2(a - f.x, b - f.y);
-}
-
 // grp_row: first token of the group inside the tile; grp_valid (1..32+): how many of its tokens exist.
 //
 // BS: `qk_scale` is without a K scale.  scale_of(t0, first, lo, hi, live, ks, vs): K and V scales of tokens lo and hi of the 16
 // that start at token t0 of the tile (`first` of the group); a token at or behind `live` does not exist and gets (1, v_ref).
 // v_ref: see above; 0 at a segment's start, where the first block sets it.
-template<bool BS, bool TWINS, typename Rows, typename Scales>
+template<bool BS, typename Rows, typename Scales>
 __device__ __forceinline__ bool process_group_e4m3(const uint32_t k_tile, const uint32_t v_tile, const Rows rows,
                                                    const int grp_row, const int grp_valid, const uint32_t (&qb)[8][2],
                                                    float (&acc)[8][4], float (&m_run)[2], float (&l_run)[2],
@@ -569,16 +559,6 @@ __device__ __forceinline__ bool process_group_e4m3(const uint32_t k_tile, const 
     const int v_lane = lane & 15;
     const uint32_t v_row = rows(grp_row + 16 * (lane >> 4) + tau16(2 * (v_lane >> 2) + (v_lane & 1) + 8 * ((v_lane >> 1) & 1)), 0);
 
-    // B fragments of two weights of the lane (MMA columns 2qd, 2qd+1): `second` only where there are no twin columns
-    auto fragments = [&](float a, float b, uint32_t& first, uint32_t& second) {
-        uint32_t w = pack_half2(a, b);
-        if constexpr (BS) {
-            const uint32_t w2 = second_term(a, b, w);
-            if constexpr (TWINS) w = qd >= 2 ? w2 : w;
-            else second = movmatrix_trans(w2);
-        }
-        first = movmatrix_trans(w);
-    };
     if constexpr (BS) {
         float rel[2][2];
         auto weigh = [&](auto outside) {              // rel of the lane's four tokens; does some token of the unit lie outside?
@@ -614,14 +594,14 @@ __device__ __forceinline__ bool process_group_e4m3(const uint32_t k_tile, const 
                     if (!(most > V_REF_MIN)) break;                            // warp-uniform, like the rest of the loop
                     const float two = power_of_two_below(fminf(most, V_REF_MAX)), back = two / v_ref;
                     const float unit = __uint_as_float(__float_as_uint(V_BOOST) + __float_as_uint(1.f) - __float_as_uint(two));
-                    uint32_t b[2][2], b2[2][2];
+                    uint32_t b[2][2];
 #pragma unroll
                     for (int hh = 0; hh < 2; hh++)
 #pragma unroll
                         for (int i = 0; i < 2; i++) {
                             float w = vs[hh][i] * unit;
                             if (w >= V_LEAST) vs[hh][i] = 0.f; else w = 0.f;
-                            fragments(pr[hh][2 * i] * w, pr[hh][2 * i + 1] * w, b[hh][i], b2[hh][i]);
+                            b[hh][i] = movmatrix_trans(pack_half2(pr[hh][2 * i] * w, pr[hh][2 * i + 1] * w));
                         }
 #pragma unroll
                     for (int mt = 0; mt < 8; mt++) {
@@ -632,10 +612,6 @@ __device__ __forceinline__ bool process_group_e4m3(const uint32_t k_tile, const 
                         float sum[4] = {0.f, 0.f, 0.f, 0.f};
                         mma_16816(sum, a0, b[0][0], b[0][1]);
                         mma_16816(sum, a1, b[1][0], b[1][1]);
-                        if constexpr (!TWINS) {
-                            mma_16816(sum, a0, b2[0][0], b2[0][1]);
-                            mma_16816(sum, a1, b2[1][0], b2[1][1]);
-                        }
 #pragma unroll
                         for (int i = 0; i < 4; i++) acc[mt][i] = fmaf(sum[i], back, acc[mt][i]);
                     }
@@ -650,11 +626,11 @@ __device__ __forceinline__ bool process_group_e4m3(const uint32_t k_tile, const 
     }
 
     // ---- 3. O^T += V^T P^T.  P^T's B fragments = transposed 8x8 blocks of the weights (MMA rows 0..7, 8..15).
-    uint32_t pb[2][2], pb2[2][2];
+    uint32_t pb[2][2];
 #pragma unroll
     for (int hh = 0; hh < 2; hh++) {
-        fragments(pr[hh][0], pr[hh][1], pb[hh][0], pb2[hh][0]);
-        fragments(pr[hh][2], pr[hh][3], pb[hh][1], pb2[hh][1]);
+        pb[hh][0] = movmatrix_trans(pack_half2(pr[hh][0], pr[hh][1]));
+        pb[hh][1] = movmatrix_trans(pack_half2(pr[hh][2], pr[hh][3]));
     }
 #pragma unroll
     for (int mt = 0; mt < 8; mt++) {
@@ -664,10 +640,6 @@ __device__ __forceinline__ bool process_group_e4m3(const uint32_t k_tile, const 
         const uint32_t a1[4] = {widen_lo(v[2]), widen_lo(v[3]), widen_hi(v[2]), widen_hi(v[3])};
         mma_16816(acc[mt], a0, pb[0][0], pb[0][1]);
         mma_16816(acc[mt], a1, pb[1][0], pb[1][1]);
-        if constexpr (BS && !TWINS) {
-            mma_16816(acc[mt], a0, pb2[0][0], pb2[0][1]);
-            mma_16816(acc[mt], a1, pb2[1][0], pb2[1][1]);
-        }
     }
     return wrote;
 }
@@ -985,9 +957,7 @@ paged_decode_kernel(const __grid_constant__ pd_params p, const __grid_constant__
     }
 
     // ================= consumer warps =================
-    constexpr bool TWINS = BS && GROUP <= 4;   // columns 4..7 of the query fragments repeat 0..3
     const int g  = lane >> 2;   // fragment row
-    const int qhead = TWINS ? g & 3 : g;
     const int qd = lane & 3;    // fragment column pair: this lane owns heads 2qd, 2qd+1
     // softmax runs in base 2; with per-head scales the factor belongs to the segment's kv head
     float qk_scale = p.sm_scale * p.k_scale * 1.4426950408889634f;
@@ -1028,9 +998,9 @@ paged_decode_kernel(const __grid_constant__ pd_params p, const __grid_constant__
         }
         if constexpr (S::HEADS > 1) {
             // head-fused: this warp's kv head is `warp`; its query rows come straight from global memory
-            const bool live = qhead < GROUP;
+            const bool live = g < GROUP;
             const __half* qrow = static_cast<const __half*>(p.q)
-                + (static_cast<size_t>(sg.x) * p.num_q_heads + warp * GROUP + (live ? qhead : 0)) * HEAD_DIM;
+                + (static_cast<size_t>(sg.x) * p.num_q_heads + warp * GROUP + (live ? g : 0)) * HEAD_DIM;
 #pragma unroll
             for (int ks = 0; ks < 8; ks++) {
                 if constexpr (FP8) {
@@ -1059,8 +1029,8 @@ paged_decode_kernel(const __grid_constant__ pd_params p, const __grid_constant__
             if (need_q && S::HEADS == 1) {
                 // column n = g is query head g of the group (zero when g >= GROUP)
                 need_q = false;
-                const bool live = qhead < GROUP;
-                const uint32_t qrow = q_slots + stage * S::Q_SLOT_BYTES + (live ? qhead : 0) * (HEAD_DIM * 2);
+                const bool live = g < GROUP;
+                const uint32_t qrow = q_slots + stage * S::Q_SLOT_BYTES + (live ? g : 0) * (HEAD_DIM * 2);
 #pragma unroll
                 for (int ks = 0; ks < 8; ks++) {
                     if constexpr (FP8) {
@@ -1108,7 +1078,7 @@ paged_decode_kernel(const __grid_constant__ pd_params p, const __grid_constant__
                             vs[i] = kv.y;
                         }
                     };
-                    wrote |= process_group_e4m3<BS, TWINS>(k_tile, v_tile, rows, grp_row, grp_valid, qb, acc, m_run, l_run, qk_scale, lane, scale_of, v_ref);
+                    wrote |= process_group_e4m3<BS>(k_tile, v_tile, rows, grp_row, grp_valid, qb, acc, m_run, l_run, qk_scale, lane, scale_of, v_ref);
                 }
                 else
                     wrote |= process_group_f16(k_tile, v_tile, rows, grp_row, grp_valid, qb, acc, m_run, l_run, qk_scale, lane);
@@ -1132,10 +1102,7 @@ paged_decode_kernel(const __grid_constant__ pd_params p, const __grid_constant__
 #pragma unroll
                 for (int mt = 0; mt < 8; mt++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        if constexpr (TWINS) acc[mt][i] += __shfl_xor_sync(0xffffffffu, acc[mt][i], 2);
-                        acc[mt][i] *= unit;
-                    }
+                    for (int i = 0; i < 4; i++) acc[mt][i] *= unit;
             }
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) {
