@@ -81,12 +81,13 @@ struct HeadScales {
 // Scales of a block-scaled e4m3 cache: float pairs (K, V) at [page][kv head][block of the page]; a block is the largest
 // power of two of tokens that divides the page size, at most 16.  The producer warp brings a tile's pairs into the
 // tile's stage with 8-byte asynchronous copies that arrive on the same barrier as the tile: 8 bytes beside 4 KB of K and V per
-// 16 tokens and head.  Against the same decode with one scale per tensor, measured on B200: 128 x 4096 tokens 163.6 us and
-// 162.1, a ragged 256 x 4100 (64 query heads) 333.8 and 329.2 (both at the copy rate of the traffic).  Steps on the
-// (row, kv head) schedule, whose warps have less time per byte, pay more: 16 x 4096 with groups of 8 32.4 us and 31.0, 32 x 1024
-// with 4 kv heads 12.9 and 12.1, 4 x 30000 with 8 kv heads 47.4 and 42.3, 1 x 200001 in pages of 64 39.7 and 39.6.  Of the 5 us
-// of 4 x 30000 half go away with constant scales that nobody loads, so half is arithmetic.  Without gain: fetching the scales
-// ahead of the products, cheaper reciprocals, prefetches into L2, plain loads by the producer's lanes one tile or four tiles ahead.
+// 16 tokens and head.  Against the same decode with one scale per tensor, measured on B200 in graphs of 20 calls: 128 x 4096
+// tokens 162.8 us and 161.6, a ragged 256 x 4100 (64 query heads) 332.5 and 329 (both at the copy rate of the traffic).  Steps on the
+// (row, kv head) schedule, whose producers have less time per byte, pay more: 16 x 4096 with groups of 8 29.9 us and 30.4, 32 x 1024
+// with 4 kv heads 13.3 and 12.2, 4 x 30000 with 8 kv heads 48.1 and 42.3, 1 x 200001 in pages of 64 41 and 40 (the difference
+// from run to run is as large).  Of 4 x 30000's 5.8 us all but 0.2 go away with constant scales that nobody copies, and 0.4 with constant
+// scales beside the copies: it is the copies.  Without gain there: prefetches into L2, plain loads by the producer's lanes one
+// tile or four tiles ahead.
 struct BlockScales {
     const float2* scales;
     int log2_block;
@@ -452,6 +453,11 @@ __device__ __forceinline__ void ldmatrix_b8_x2_trans(uint32_t (&r)[4], uint32_t 
 // its product joins the accumulators in fp32, so that an outlier in one block takes no bits from the others.  Where
 // that is every unit (scales spread over 2^18 at random) 128 x 4096 tokens take 167 us instead of 163.5, 64 x 2048 in pages of 5,
 // with a scale per token, 132 instead of 112.
+//
+// The weights are rounded to fp16 once, as in the decodes without block scales: an error of 2.4e-4 relative against 64 bits where the
+// rounding of the fp16 output alone is 2.07e-4.  A second fp16 term for the rest of each weight, in the MMA columns that
+// groups of up to four query heads leave free or in an MMA of its own, brought 2.07e-4 and no difference in short loops, but in
+// loops of seconds, at the power cap, 171.2 us instead of 167.9 (128 x 4096) and 367 instead of 344 (256 x 4100 with groups of 8).
 constexpr float V_BOOST = 8192.f, V_LEAST = 32.f;
 constexpr float V_REF_MIN = 0x1p-64f, V_REF_MAX = 0x1p126f;   // outputs are fp16: smaller scales are invisible
 __device__ __forceinline__ float power_of_two_below(float x) {   // x positive and normal
@@ -1258,8 +1264,8 @@ paged_decode_kernel(const __grid_constant__ pd_params p, const __grid_constant__
 // ROW_ITEMS = true: the plan's work items are rows (head-fused tiles).
 constexpr int MERGE_WIDE_MIN = 8;
 // One (row, query head) pair by the four warps of a CTA; s0, s1: the pair's segment range.
-// WARPS, LOADS: warps of the CTA and pieces each has in flight.  The block-scaled decode takes 16 warps with four pieces each
-// while that many warps fit at once (a merge of 71 pieces is two rounds of loads instead of five).
+// WARPS: warps of the CTA; each has four pieces in flight.  The block-scaled decode takes 16 warps while that many
+// fit at once (a merge of 71 pieces is two rounds of loads instead of five).
 template<int GROUP, bool ROW_ITEMS, int WARPS = 4>
 __device__ __forceinline__ void merge_pair(const pd_params& p, int idx, int s0, int s1, int seg_limit, float4 (*part_num)[32], float* part_den)
 {

@@ -126,7 +126,8 @@ void launch_dependent(Kernel kernel, int blocks, const pd_params& p, int seg_lim
     cudaLaunchKernelEx(&cfg, kernel, p, seg_limit);
 }
 // A block-scaled decode of few (row, head) pairs, and so of many pieces each, merges them with 16 warps per pair: two such
-// CTAs fit on an SM.
+// CTAs fit on an SM (1 x 50000 tokens with one kv head: 16.2 us with four warps, 12.6 with 16).  The other decodes read the same
+// partials and would gain as much, but 16 warps add them up in another order: they keep four, and with them their results bit for bit.
 constexpr int WIDE_MERGE_PAIRS = 148 * 2, WIDE_MERGE_WARPS = 16;
 template<int GROUP>
 void launch_merge(const pd_params& p, int seg_limit, bool scaled, cudaStream_t stream) {
@@ -1063,11 +1064,12 @@ struct Selection {
     int schedule;                  // 0 the caller's plan, 1 head-fused rows, 2 the caller's plan in unequal shares
     unsigned long long* stats;
 };
-// scaled: a block-scaled decode.  On the (row, kv head) schedule its 8-byte loads of scales per 2 KB box cost up to 10 %, on the
+// scaled: a block-scaled decode.  On the (row, kv head) schedule its 8-byte copies of scales per 2 KB box cost up to 14 %, on the
 // head-fused one 1 %, so it is head-fused for fewer rows too: what it gains grows with a CTA's tiles, what the merge costs with
-// a row's pieces.  Rows cut in up to 24 pieces, and two tiles per CTA for every three pieces (16 x 10000 tokens, 10 pieces and 34
-// tiles: 62.0 us and 56.3 head-fused; 16 x 2000, 10 and 7: 19.7 and 17.8; 8 x 30000, 19 and 51: 86.7 and 81.2; 8 x 8000, 19 and 14:
-// 28.7 and 28.8; on the other side 16 x 1000, 10 and 3: 12.8 and 13.8; 4 x 30000, 37 and 25: 47.1 and 47.8).
+// a row's pieces.  Rows cut in up to 24 pieces, and two tiles per CTA for every three pieces.  Measured with 8 kv heads, the only
+// ones that have this choice: 16 x 10000 tokens (10 pieces, 34 tiles) 63.1 us and 56.8 head-fused; 12 x 12000 57.7 and 51.9; 24 x 2000 25.7 and
+// 24.8; 16 x 2000 (10, 7) 19.8 and 18.0; 8 x 30000 (19, 51) 88.3 and 81.7; at the border 8 x 8000 (19, 14) 29.3 and 29.7; on the other side
+// 16 x 1000 (10, 3) 12.9 and 13.8, 4 x 30000 (37, 25) 48.2 and 47.9.
 constexpr int SCALED_MOST_PIECES = 24;
 Selection select_schedule(int dtype, const pd_params* p, const KernelInfo* k, bool gathered, bool scaled, pd_params* scratch) {
     Selection sel{p, k, 1, 0, nullptr};

@@ -36,7 +36,7 @@ constexpr int ROWS_THREADS = ROWS_WARPS * 32;
 constexpr int ROWS_SLOTS   = 4;             // units (four heads, 1 KB) a warp has in flight: 8 measured the same
 constexpr int MAX_FREQS    = 64;
 constexpr int MAX_BLOCK    = 16;            // tokens that share a scale, at most
-// block scales are powers of two in [2^-32, 2^8]: 2^-32 * 448 is below the smallest fp16 number, 2^8 * 448 above the largest
+// block scales are powers of two in [2^-32, 2^8]: under 2^-32 the smallest fp16 number, 2^-24, is 256; 2^8 * 448 is above the largest
 constexpr int MIN_SCALE_EXP = -32, MAX_SCALE_EXP = 8;
 
 constexpr unsigned ST_APPEND_RANGE = 7;     // a token's place lies outside the block table or its page outside the pool
