@@ -223,8 +223,8 @@ int pd_paged_decode_scaled(int dtype, const pd_params* p, int num_pages, const f
 /* The same decode over an e4m3 cache with one scale per (block of tokens, kv head) for K and for V, as
  * pd_append_qkv and a cache with pd_cache_set_block_scales leave it.  No counterpart in the reference.
  * d_block_scales: device floats [num_pages][num_kv_heads][page_size / block][2] (K, V), 8-byte aligned, block =
- * pd_scale_block_tokens(page_size); positive and finite (0: nothing was ever written there).  p->k_scale and
- * p->v_scale are ignored.  num_pages must be positive: scales of pages outside [0, num_pages) are not read. */
+ * pd_scale_block_tokens(page_size); positive and finite (0: nothing was ever written there, K and V count as zeros),
+ * in any ratio to each other.  p->k_scale and p->v_scale are ignored.  num_pages must be positive: scales of pages outside [0, num_pages) are not read. */
 int pd_paged_decode_block_scaled(int dtype, const pd_params* p, int num_pages, const float* d_block_scales, void* stream);
 
 /* What a decode of these params would launch (no counterpart in the reference, which has one kernel shape):
@@ -440,6 +440,8 @@ int    pd_cache_append_batch(pd_cache* c, int count, const int* slots, const voi
  * the fp16 query rows.  No counterpart in the reference. */
 int    pd_cache_append_qkv(pd_cache* c, int count, const int* slots, const int* n, const pd_qkv* x, const pd_rope* rope,
                            void* q_out, void* stream);
+/* Waits for a batched append that is still on its way.  The slot's device length is zeroed behind what the default stream
+ * holds; later appends and pd_cache_plan_device wait for that on their own streams (a captured plan cannot). */
 int    pd_cache_release(pd_cache* c, int slot);
 /* Per-kv-head scales for an fp8 cache (host arrays of num_kv_heads positive floats; both NULL: back to
  * the per-tensor scales of the config).  Every later append quantises and every later run dequantises

@@ -19,7 +19,7 @@
 // Bound: memory, one read of the rows and one write of the results.  Measured on B200 against that traffic at the
 // measured copy rate (6.55 TB/s): 8192 bf16 rows of 40 heads with norm 28.8 us (89 %), 65536 of them 201 us (102 %), 20001
 // rows of 72 heads 113 us (99 %), prompts of 33,000 rows of 80 heads into an fp16 cache 206 us (100 %), ragged chunks of
-// 12,000 rows into an e4m3 cache 47 us (88 %), of 15,500 into a block-scaled one 65 us (82 %; 87 % at four times the rows); one
+// 12,000 rows into an e4m3 cache 48 us (87 %), of 15,500 into a block-scaled one 65 us (82 %; 87 % at four times the rows); one
 // row 2.3 us, a launch.  What is missing at the smaller sizes is 3 us of first loads and last stores.
 
 #include <cuda_bf16.h>
