@@ -448,18 +448,26 @@ __device__ __forceinline__ void ldmatrix_b8_x2_trans(uint32_t (&r)[4], uint32_t 
 // Block-scaled cache: the accumulators are in units of v_ref / V_BOOST, v_ref a power of two that the warp raises to the
 // largest V scale it has met in the segment (rescaling is exact).  A token's weight is p * rel, rel = vs * V_BOOST / v_ref.
 // p is in [0, 1], and as long as rel is in [V_LEAST, 2 V_BOOST) the fp16 operand p * rel neither overflows nor loses bits to
-// fp16's subnormals for any p >= 2^-19.  A unit with a scale below that range (one block's V 2^8 times smaller than
-// another's in the same segment) is done in passes instead, one per range of scales: a pass has its own reference and
-// its product joins the accumulators in fp32, so that an outlier in one block takes no bits from the others.  Where
-// that is every unit (scales spread over 2^18 at random) 128 x 4096 tokens take 167 us instead of 163.5, 64 x 2048 in pages of 5,
-// with a scale per token, 132 instead of 112.
+// fp16's subnormals for any p >= 2^-19.  Two kinds of units are done in passes instead:
+//  * those with a scale below that range (one block's V 2^8 times smaller than another's in the same segment);
+//  * all units once the segment's scales are more than V_WIDE apart, because tokens of smaller p then count too if their scale
+//    is large.
+// A pass takes, per query head, the weights within 2^27 of the largest one left, in a power of two of their own, and its
+// product joins the accumulators in fp32: an outlier in one block takes no bits from the others, nor they from it.
+// Where that is every unit (scales spread over 2^18 at random) 128 x 4096 tokens take 177 us instead of 163, 64 x 2048 in
+// pages of 5, with a scale per token, 115.5 instead of 111.5.
 //
 // The weights are rounded to fp16 once, as in the decodes without block scales: an error of 2.4e-4 relative against 64 bits where the
 // rounding of the fp16 output alone is 2.07e-4.  A second fp16 term for the rest of each weight, in the MMA columns that
 // groups of up to four query heads leave free or in an MMA of its own, brought 2.07e-4 and no difference in short loops, but in
 // loops of seconds, at the power cap, 171.2 us instead of 167.9 (128 x 4096) and 367 instead of 344 (256 x 4100 with groups of 8).
 constexpr float V_BOOST = 8192.f, V_LEAST = 32.f;
-constexpr float V_REF_MIN = 0x1p-64f, V_REF_MAX = 0x1p126f;   // outputs are fp16: smaller scales are invisible
+constexpr float V_WIDE = 0x1p16f;
+constexpr float V_REF_MIN = 0x1p-40f, V_REF_MAX = 0x1p40f;    // smaller scales are invisible in fp16 outputs; larger ones go in passes
+struct VScales {
+    float ref = 0.f;    // v_ref; 0 at a segment's start, where the first block sets both
+    float low = 0.f;    // no live scale met so far was smaller (but for zeros)
+};
 __device__ __forceinline__ float power_of_two_below(float x) {   // x positive and normal
     return __uint_as_float(__float_as_uint(x) & 0x7f800000u);
 }
@@ -467,14 +475,13 @@ __device__ __forceinline__ float power_of_two_below(float x) {   // x positive a
 // grp_row: first token of the group inside the tile; grp_valid (1..32+): how many of its tokens exist.
 //
 // BS: `qk_scale` is without a K scale.  scale_of(t0, first, lo, hi, live, ks, vs): K and V scales of tokens lo and hi of the 16
-// that start at token t0 of the tile (`first` of the group); a token at or behind `live` does not exist and gets (1, v_ref).
-// v_ref: see above; 0 at a segment's start, where the first block sets it.
-template<bool BS, typename Rows, typename Scales>
+// that start at token t0 of the tile (`first` of the group); a token at or behind `live` does not exist and gets (1, v.ref).
+template<int GROUP, bool BS, typename Rows, typename Scales>
 __device__ __forceinline__ bool process_group_e4m3(const uint32_t k_tile, const uint32_t v_tile, const Rows rows,
                                                    const int grp_row, const int grp_valid, const uint32_t (&qb)[8][2],
                                                    float (&acc)[8][4], float (&m_run)[2], float (&l_run)[2],
                                                    const float qk_scale, const int lane, const Scales scale_of,
-                                                   float& v_ref)
+                                                   VScales& v)
 {
     const int g = lane >> 2, qd = lane & 3;
     bool wrote = false;
@@ -511,10 +518,11 @@ __device__ __forceinline__ bool process_group_e4m3(const uint32_t k_tile, const 
         }
         if constexpr (BS) {
             float ks[2];
-            if (hh == 0 && v_ref == 0.f) {            // warp-uniform
+            if (hh == 0 && v.ref == 0.f) {            // warp-uniform
                 float first[2];
                 scale_of(grp_row, 0, 0, 0, grp_valid, ks, first);
-                v_ref = power_of_two_below(fminf(fmaxf(first[0], V_REF_MIN), V_REF_MAX));
+                v.low = power_of_two_below(fminf(fmaxf(first[0], V_REF_MIN), V_REF_MAX));
+                v.ref = fminf(4.f * v.low, V_REF_MAX);                         // room for scales that are a little larger
             }
             scale_of(grp_row + 16 * hh, 16 * hh, tok_lo, tok_hi, grp_valid, ks, vs[hh]);
 #pragma unroll
@@ -568,7 +576,7 @@ __device__ __forceinline__ bool process_group_e4m3(const uint32_t k_tile, const 
     if constexpr (BS) {
         float rel[2][2];
         auto weigh = [&](auto outside) {              // rel of the lane's four tokens; does some token of the unit lie outside?
-            const float unit = __uint_as_float(__float_as_uint(V_BOOST) + __float_as_uint(1.f) - __float_as_uint(v_ref));   // V_BOOST / v_ref
+            const float unit = __uint_as_float(__float_as_uint(V_BOOST) + __float_as_uint(1.f) - __float_as_uint(v.ref));   // V_BOOST / v.ref
             bool out = false;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -578,49 +586,82 @@ __device__ __forceinline__ bool process_group_e4m3(const uint32_t k_tile, const 
             return __any_sync(0xffffffffu, out);
         };
         // (positive floats are ordered like their bits; zeros and NaN lie outside too)
-        if (weigh([](float r) { return __float_as_uint(r) - __float_as_uint(V_LEAST) >= __float_as_uint(2.f * V_BOOST) - __float_as_uint(V_LEAST); })) {
-            auto largest = [&](const float (&s)[2][2]) {
-                float top = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
+        const bool outside = weigh([](float r) { return __float_as_uint(r) - __float_as_uint(V_LEAST) >= __float_as_uint(2.f * V_BOOST) - __float_as_uint(V_LEAST); });
+        if (__builtin_expect(outside || v.ref > V_WIDE * v.low, 0)) {
+            float top = fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[1][0], vs[1][1])), low = INFINITY;
 #pragma unroll
-                for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                return top;
-            };
-            const float top = power_of_two_below(fminf(fmaxf(largest(vs), v_ref), V_REF_MAX));
-            const float down = v_ref / top;
+            for (int i = 0; i < 4; i++)
+                if (vs[i >> 1][i & 1] > 0.f) low = fminf(low, vs[i >> 1][i & 1]);
 #pragma unroll
-            for (int mt = 0; mt < 8; mt++)
+            for (int o = 4; o < 32; o <<= 1) {
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+            }
+            top = power_of_two_below(fminf(fmaxf(top, v.ref), V_REF_MAX));
+            if (top > v.ref) {
+                low = fminf(low, v.ref * (V_LEAST / V_BOOST));                 // of the units that did not come here
+                const float down = v.ref / top;
 #pragma unroll
-                for (int i = 0; i < 4; i++) acc[mt][i] *= down;
-            v_ref = top;
-            if (weigh([](float r) { return r < V_LEAST && r != 0.f; })) {      // (a block nothing was ever written to weighs 0)
-                // Tokens of one range of scales after the other, from the largest down: each pass takes at least the block with
-                // the largest scale left.
-                for (;;) {
-                    const float most = largest(vs);
-                    if (!(most > V_REF_MIN)) break;                            // warp-uniform, like the rest of the loop
-                    const float two = power_of_two_below(fminf(most, V_REF_MAX)), back = two / v_ref;
-                    const float unit = __uint_as_float(__float_as_uint(V_BOOST) + __float_as_uint(1.f) - __float_as_uint(two));
+                for (int mt = 0; mt < 8; mt++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) acc[mt][i] *= down;
+                v.ref = top;
+            }
+            v.low = fminf(v.low, fmaxf(low, V_REF_MIN));
+            if (weigh([](float r) { return !(r < 2.f * V_BOOST) || (r < V_LEAST && r != 0.f); }) || v.ref > V_WIDE * v.low) {
+                // per column (query head 2qd, 2qd + 1): largest weight left, over all 32 tokens
+                float w[2][4] = {}, most[2];
+                auto find_most = [&]() {
+                    most[0] = fmaxf(fmaxf(w[0][0], w[0][2]), fmaxf(w[1][0], w[1][2]));
+                    most[1] = fmaxf(fmaxf(w[0][1], w[0][3]), fmaxf(w[1][1], w[1][3]));
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) {
+                        most[0] = fmaxf(most[0], __shfl_xor_sync(0xffffffffu, most[0], o));
+                        most[1] = fmaxf(most[1], __shfl_xor_sync(0xffffffffu, most[1], o));
+                    }
+                };
+#pragma unroll
+                for (int i = 0; i < 8; i++) w[i >> 2][i & 3] = 2 * qd + (i & 1) < GROUP ? pr[i >> 2][i & 3] * rel[i >> 2][i >> 1 & 1] : 0.f;
+                find_most();
+                // a token that has neither 2^-60 of the largest p nor 2^-60 of the unit's largest weight is left out
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    if (!(pr[i >> 2][i & 3] > 0x1p-60f || w[i >> 2][i & 3] > 0x1p-60f * most[i & 1])) w[i >> 2][i & 3] = 0.f;
+                while (__any_sync(0xffffffffu, most[0] > 0.f || most[1] > 0.f)) {
+                    float to[2], back[2];
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        // (within these bounds, the largest weight left is taken whatever it is, so the passes end)
+                        const float two = power_of_two_below(fminf(fmaxf(most[h], 0x1p-100f), 0x1p110f));
+                        to[h] = 0x1p14f / two;
+                        back[h] = two * 0x1p-14f;
+                    }
                     uint32_t b[2][2];
 #pragma unroll
                     for (int hh = 0; hh < 2; hh++)
 #pragma unroll
                         for (int i = 0; i < 2; i++) {
-                            float w = vs[hh][i] * unit;
-                            if (w >= V_LEAST) vs[hh][i] = 0.f; else w = 0.f;
-                            b[hh][i] = movmatrix_trans(pack_half2(pr[hh][2 * i] * w, pr[hh][2 * i + 1] * w));
+                            float x2[2];
+#pragma unroll
+                            for (int h = 0; h < 2; h++) {
+                                x2[h] = w[hh][2 * i + h] * to[h];
+                                if (x2[h] >= 0x1p-13f) w[hh][2 * i + h] = 0.f; else x2[h] = 0.f;
+                            }
+                            b[hh][i] = movmatrix_trans(pack_half2(x2[0], x2[1]));
                         }
 #pragma unroll
                     for (int mt = 0; mt < 8; mt++) {
-                        uint32_t v[4];
-                        ldmatrix_b8_x2_trans(v, v_tile + swz(v_row, mt));
-                        const uint32_t a0[4] = {widen_lo(v[0]), widen_lo(v[1]), widen_hi(v[0]), widen_hi(v[1])};
-                        const uint32_t a1[4] = {widen_lo(v[2]), widen_lo(v[3]), widen_hi(v[2]), widen_hi(v[3])};
+                        uint32_t d[4];
+                        ldmatrix_b8_x2_trans(d, v_tile + swz(v_row, mt));
+                        const uint32_t a0[4] = {widen_lo(d[0]), widen_lo(d[1]), widen_hi(d[0]), widen_hi(d[1])};
+                        const uint32_t a1[4] = {widen_lo(d[2]), widen_lo(d[3]), widen_hi(d[2]), widen_hi(d[3])};
                         float sum[4] = {0.f, 0.f, 0.f, 0.f};
                         mma_16816(sum, a0, b[0][0], b[0][1]);
                         mma_16816(sum, a1, b[1][0], b[1][1]);
 #pragma unroll
-                        for (int i = 0; i < 4; i++) acc[mt][i] = fmaf(sum[i], back, acc[mt][i]);
+                        for (int i = 0; i < 4; i++) acc[mt][i] = fmaf(sum[i], back[i & 1], acc[mt][i]);
                     }
+                    find_most();
                 }
                 return wrote;
             }
@@ -968,7 +1009,7 @@ paged_decode_kernel(const __grid_constant__ pd_params p, const __grid_constant__
     // softmax runs in base 2; with per-head scales the factor belongs to the segment's kv head
     float qk_scale = p.sm_scale * p.k_scale * 1.4426950408889634f;
     float v_scale  = p.v_scale;
-    float v_ref = 0.f;          // block-scaled: unit of the accumulators, see V_BOOST; v_scale is then 1 until a segment's end
+    VScales v_scales;           // block-scaled: unit of the accumulators, see V_BOOST; v_scale is then 1
     if constexpr (BS) { qk_scale = p.sm_scale * 1.4426950408889634f; v_scale = 1.f; }
     if constexpr (S::HEADS > 1 && !BS) {
         if (hs.k) qk_scale = p.sm_scale * __ldg(hs.k + warp) * 1.4426950408889634f;
@@ -1026,7 +1067,7 @@ paged_decode_kernel(const __grid_constant__ pd_params p, const __grid_constant__
         for (int mt = 0; mt < 8; mt++) acc[mt][0] = acc[mt][1] = acc[mt][2] = acc[mt][3] = 0.f;
         m_run[0] = m_run[1] = -INFINITY;
         l_run[0] = l_run[1] = 0.f;
-        v_ref = 0.f;
+        v_scales = VScales{};
 
         for (int tok = sg.z; tok < sg.w; tok += S::TILE) {
             const int stage = c_stage;
@@ -1075,7 +1116,7 @@ paged_decode_kernel(const __grid_constant__ pd_params p, const __grid_constant__
                         for (int i = 0; i < 2; i++) {
                             if (i == 1 && bs.log2_block == 4) { ks[1] = ks[0]; vs[1] = vs[0]; break; }
                             const int in_half = bs.log2_block == 4 ? 0 : i ? hi : lo;
-                            float2 kv = make_float2(1.f, v_ref);
+                            float2 kv = make_float2(1.f, v_scales.ref);
                             if (first + in_half < live) {
                                 const uint2 raw = lds64(slot + (((t0 + in_half) >> bs.log2_block) * S::HEADS + box_head) * 8);
                                 kv = make_float2(__uint_as_float(raw.x), __uint_as_float(raw.y));
@@ -1084,7 +1125,7 @@ paged_decode_kernel(const __grid_constant__ pd_params p, const __grid_constant__
                             vs[i] = kv.y;
                         }
                     };
-                    wrote |= process_group_e4m3<BS>(k_tile, v_tile, rows, grp_row, grp_valid, qb, acc, m_run, l_run, qk_scale, lane, scale_of, v_ref);
+                    wrote |= process_group_e4m3<GROUP, BS>(k_tile, v_tile, rows, grp_row, grp_valid, qb, acc, m_run, l_run, qk_scale, lane, scale_of, v_scales);
                 }
                 else
                     wrote |= process_group_f16(k_tile, v_tile, rows, grp_row, grp_valid, qb, acc, m_run, l_run, qk_scale, lane);
@@ -1104,7 +1145,7 @@ paged_decode_kernel(const __grid_constant__ pd_params p, const __grid_constant__
         {
             float l[2] = {l_run[0], l_run[1]};
             if constexpr (BS) {
-                const float unit = v_ref / V_BOOST;
+                const float unit = v_scales.ref / V_BOOST;
 #pragma unroll
                 for (int mt = 0; mt < 8; mt++)
 #pragma unroll

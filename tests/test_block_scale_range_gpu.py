@@ -54,7 +54,9 @@ def check(torch, pa, q, kc, vc, scales, table, lens, ps, ctas):
         pa.set_head_fused(mode)
 
 
-@pytest.mark.parametrize("power, share", [(4, 0.5), (7, 0.5), (10, 0.5), (12, 0.1), (12, 0.5), (14, 0.9), (18, 0.5), (28, 0.5)])
+@pytest.mark.parametrize("power, share", [(4, 0.5), (7, 0.5), (10, 0.5), (12, 0.1), (12, 0.5), (14, 0.9), (18, 0.5), (28, 0.5),
+                                          # an outlier that counts although it has next to no share
+                                          (18, 2.0 ** -17), (28, 2.0 ** -27), (28, 2.0 ** -35)])
 @pytest.mark.parametrize("one_sign", [False, True])
 @pytest.mark.parametrize("ps, hq, hkv, lens, at, ctas", [
     (16, 32, 8, [4096, 40, 1], 5, 0), (64, 8, 8, [1500, 700], 900, 3), (16, 8, 1, [2000], 1999, 1), (24, 16, 8, [500, 77], 12, 2), (8, 4, 4, [333], 100, 0),
@@ -87,5 +89,21 @@ def test_scales_all_over_the_range(ps, hq, hkv, lens, ctas, power_of_two, torch_
         scales[..., 0] *= rng.uniform(0.5, 2, scales.shape[:3])
     token_scale = np.repeat(scales[..., 1], ro.block_tokens(ps), axis=2)
     bytes_[1][..., :64][token_scale > 2.0 ** -12] = 0
+    q = rng.standard_normal((len(lens), hq, 128)).astype(np.float16)
+    check(torch, pa, q, *(torch.from_numpy(x).cuda() for x in (*bytes_, scales)), table, lens, ps, ctas)
+
+
+@pytest.mark.parametrize("ps, hq, hkv, lens, ctas", [(16, 32, 8, [100, 700, 16], 0), (8, 8, 4, [77, 300], 3), (3, 16, 8, [40, 2], 0)])
+def test_scale_zero_and_scales_far_outside_the_appends_range(ps, hq, hkv, lens, ctas, torch_cuda, pa):
+    """Blocks of scale 0 count as zeros whatever their bytes; blocks of huge scales whose V bytes are zeros take no bits either; V
+    scales that fp16 outputs cannot show."""
+    torch = torch_cuda
+    rng = np.random.default_rng(ps)
+    table, pages, bytes_, scales = random_cache(rng, lens, hkv, ps, 1)
+    kind = rng.integers(0, 5, scales.shape[:3])
+    scales[kind == 0] = 0
+    scales[..., 1][kind == 1] = 2.0 ** rng.uniform(20, 125, (kind == 1).sum())
+    scales[..., 1][kind == 2] = 2.0 ** rng.uniform(-120, -33, (kind == 2).sum())
+    bytes_[1][np.repeat(kind, ro.block_tokens(ps), axis=2) == 1] = 0
     q = rng.standard_normal((len(lens), hq, 128)).astype(np.float16)
     check(torch, pa, q, *(torch.from_numpy(x).cuda() for x in (*bytes_, scales)), table, lens, ps, ctas)
