@@ -1646,10 +1646,7 @@ namespace {
 // release() queues its zero of the slot's device length on the default stream, behind the kernels there that may still read the
 // old one; what writes or reads the lengths next waits for it on its own stream.
 int wait_for_release(pd_cache* c, cudaStream_t stream) {
-    if (!c->release_pending) return PD_OK;
-    PD_CUDA(cudaStreamWaitEvent(stream, c->released, 0));
-    if (cudaEventQuery(c->released) == cudaSuccess) c->release_pending = false;
-    else cudaGetLastError();
+    if (c->release_pending) PD_CUDA(cudaStreamWaitEvent(stream, c->released, 0));
     return PD_OK;
 }
 // The cache as the target of an append; the caller adds which sequences.
@@ -1734,7 +1731,7 @@ int pd_cache_append(pd_cache* c, int slot, const void* d_k, const void* d_v, int
         return rc;
     // As in the reference (src/decode/paged_kv_cache.cu:133-134) the call returns with the tokens in place.
     PD_CUDA(cudaStreamSynchronize(stream));
-    c->batch_pending = false;              // waited for above
+    c->batch_pending = c->release_pending = false;              // waited for above
     return PD_OK;
 }
 
@@ -1844,6 +1841,10 @@ int append_batch_impl(pd_cache* c, int count, const int* slots, const void* cons
     // the previous batch's kernels, perhaps on another stream, still read the device copy of their lists
     if (c->batch_pending) PD_CUDA(cudaStreamWaitEvent(stream, c->batch_done, 0));
     if (int rc = wait_for_release(c, stream)) return rc;
+    if (c->release_pending) {              // no later call needs to wait for what has happened
+        if (cudaEventQuery(c->released) == cudaSuccess) c->release_pending = false;
+        else cudaGetLastError();
+    }
     PD_CUDA(cudaMemcpyAsync(c->batch_device, c->batch_staging, total, cudaMemcpyHostToDevice, stream));
     PD_CUDA(cudaEventRecord(c->batch_staged, stream));
     char* d = static_cast<char*>(c->batch_device);
@@ -1999,8 +2000,11 @@ int pd_cache_plan_device(pd_cache* c, const int* d_slot_ids, int batch, int num_
         return set_error(PD_INVALID_ARGUMENT, "plan_device: batch exceeds the cache's slots");
     // (a capture cannot wait for what was queued before it; its replays come after)
     cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-    if (c->release_pending && cudaStreamIsCapturing(static_cast<cudaStream_t>(stream), &capture) == cudaSuccess &&
-        capture == cudaStreamCaptureStatusNone)
+    if (c->release_pending && cudaStreamIsCapturing(static_cast<cudaStream_t>(stream), &capture) != cudaSuccess) {
+        cudaGetLastError();
+        capture = cudaStreamCaptureStatusActive;
+    }
+    if (capture == cudaStreamCaptureStatusNone)
         if (int rc = wait_for_release(c, static_cast<cudaStream_t>(stream))) return rc;
     if (int rc = pd_device_plan_build(c->device_plan, c->cfg.dtype, c->d_seq_lens, d_slot_ids, batch, num_q_heads,
                                       c->cfg.num_kv_heads, c->cfg.head_dim, num_ctas, stream))

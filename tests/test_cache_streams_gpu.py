@@ -173,3 +173,32 @@ def test_a_length_past_31_bits_is_refused(dtype, blocks, torch_cuda, pa):
         with pytest.raises(pa.LengthError):
             c.append_batch([slot], [x], [x], [n])
     assert c.seq_len(slot) == 3 and c.free_pages() == 7
+
+
+def test_a_device_plan_is_captured_behind_a_release(torch_cuda, pa):
+    """The capture neither fails on the wait for the release's zero nor leaves it out of the replays' past."""
+    torch = torch_cuda
+    side = torch.cuda.Stream()
+    x = torch.ones(40, 2, 128, dtype=torch.float16, device="cuda")
+    q, out = torch.ones(2, 4, 128, dtype=torch.float16, device="cuda"), torch.zeros(2, 4, 128, dtype=torch.float16, device="cuda")
+    c = new_cache(pa, dtype=0)
+    assert [c.admit(), c.admit()] == [0, 1] and c.append(0, x, x, 40) and c.append(1, x, x, 20)
+    c.plan_device(2, 4, stream=side.cuda_stream)
+    c.run(q, out, side.cuda_stream)                              # first use: buffers are sized
+    torch.cuda.synchronize()
+    c.release(0)
+    torch.cuda.synchronize()
+    out.fill_(7)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        c.plan_device(2, 4, stream=side.cuda_stream)
+        c.run(q, out, side.cuda_stream)
+    g.replay()
+    torch.cuda.synchronize()
+    assert (out[0] == 7).all() and (out[1] == 1).all()
+    assert c.admit() == 0 and c.append_batch([0], [x], [x], [33], side.cuda_stream)
+    torch.cuda.synchronize()
+    g.replay()
+    torch.cuda.synchronize()
+    assert pa.kernel_status() == 0 and (out == 1).all()
